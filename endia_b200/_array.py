@@ -44,11 +44,12 @@ def alloc(n_floats):
 
 
 def drop_operand_parts(arr):
-    """Forget the cached GEMM operand parts (tf32 low part, bf16 split) of an array whose storage
-    has just been rewritten in place."""
+    """Forget the cached GEMM operand parts (tf32 low part, bf16 split) and the 8-bit form of an array
+    whose storage has just been rewritten in place."""
     base = arr.base()
     base._tf32_lo = None
     base._pair16 = None
+    base._kept8 = None
 
 
 def await_pending(arr):

@@ -67,6 +67,7 @@ class FftFusion(C.Structure):
 # status codes
 OK, EINVAL, ECUDA, ENODEV, ENOMEM, ESHAPE, EPOW2, ETIMEOUT, ELIMIT = 0, -1, -2, -3, -4, -5, -6, -7, -8
 ACT_NONE, ACT_RELU, ACT_TANH, ACT_SIGMOID = 0, 1, 2, 3
+LOSS_MEAN, LOSS_SUM, LOSS_NONE = 0, 1, 2
 GEMM_AUTO, GEMM_FFMA, GEMM_3XTF32, GEMM_TF32_BF16X2 = 0, 1, 2, 3
 (UN_COPY, UN_NEG, UN_RELU, UN_TANH, UN_SIGMOID, UN_SQUARE, UN_SQRT, UN_ABS, UN_SIGN, UN_CONJ,
  UN_EXP, UN_LOG, UN_SIN, UN_COS, UN_RECIPROCAL, UN_SINH, UN_COSH, UN_TAN, UN_ASIN, UN_ACOS,
@@ -122,6 +123,18 @@ SIGNATURES = {
     "endia_b200_act_bwd_colsum_scratch_bytes": (_sz, [_i64, _i64]),
     "endia_b200_act_bwd_colsum": (C.c_int, [C.c_int, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp]),
     "endia_b200_act_bwd_colsum_parts": (C.c_int, [C.c_int, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp]),
+    "endia_b200_linear_ce_state_bytes": (_sz, [_i64]),
+    "endia_b200_linear_ce_scratch_bytes": (_sz, [_i64, _i64, _i64, _i32]),
+    "endia_b200_linear_ce_fwd": (C.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp]),
+    "endia_b200_linear_ce_bwd": (C.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp,
+                                           _vp, _vp, _vp]),
+    "endia_b200_keep8_bytes": (_sz, [_i64, _i64]),
+    "endia_b200_keep8": (C.c_int, [_vp, _i64, _i64, _i64, _i32, _vp, _vp]),
+    "endia_b200_keep8_read": (C.c_int, [_vp, _i64, _i64, _vp, _vp]),
+    "endia_b200_linear_keep_scratch_bytes": (_sz, [_i64, _i64, _i64, _i32]),
+    "endia_b200_linear_keep_fwd": (C.c_int, [_vp, _i64, _vp, _i64, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _i32, _vp, _vp]),
+    "endia_b200_linear_keep_bwd": (C.c_int, [_vp, _vp, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp,
+                                             _vp]),
     "endia_b200_adam_step_multi": (C.c_int, [_i32, C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_vp),
                                              C.POINTER(_vp), C.POINTER(_i64), _f32, _f32, _f32,
                                              _f32, _f32, _f32, _vp]),

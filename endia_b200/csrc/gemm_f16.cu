@@ -1,0 +1,651 @@
+// fp32-accurate products from fp16 pairs (see gemm_f16.cuh) and the passes that make the pairs.
+//
+// One persistent kernel of CTA pairs (cta_group::2), 256 x 256 tiles, as the framework's other two-CTA
+// product, but with another division of the work, because what limits accuracy there is the
+// accumulator: tensor memory adds with rounding toward zero, a bias that grows with the number of
+// adds (1e-5 of the result after 2048 of K). Here an accumulator lives for ONE stage of 64 of K:
+//   - the eight correction MMAs first, into an empty accumulator (they are 2^-11 of the result, so
+//     their truncation is too), then the four MMAs of hi*hi: four truncating adds in all;
+//   - the epilogue warps add it to the tile's sums, which they hold in registers (128 a thread) with
+//     round to nearest, while the MMAs of the next stage fill the other half of tensor memory.
+// Per stage the tensor pipe is busy for 12 x 128 = 1536 cycles; the drain of 256 columns by eight warps
+// takes about a third of that, so it costs no tensor time. What it buys: errors of 2e-7 instead of
+// 1e-5 at K = 4096, at 3 fp16 MMAs per product (tf32 + 2 bf16 take the time of 4).
+//   warp 0: TMA producer (one lane), warp 1: MMA issuer (one lane of the leader CTA),
+//   warps 2-9: sums, epilogue and stores (lane quarter warp & 3, column half (warp - 2) >> 2).
+// Every wait is bounded; a wait that gives up records a code, the CTA drains its copies and returns.
+#include "gemm_f16.cuh"
+#include "gemm.cuh"
+#include "tc_ptx.cuh"
+
+namespace eb {
+
+constexpr int F16_BK = 64;                       // one stage: 64 of K, 128 bytes per K-major row
+constexpr uint32_t F16_TILE = 128 * F16_BK * 2;  // bytes of one [128 x 64] fp16 tile
+constexpr int F16_EPI_WARPS = 8;
+
+struct F16Maps {
+  CUtensorMap a_hi, a_lo, b_hi, b_lo;
+  CUtensorMap c;           // F16_STORE: C or the work space, boxes of [32 rows][32 floats]
+  CUtensorMap d_hi, d_lo;  // F16_DLOGITS: boxes of [32 rows][64 halfs]
+};
+
+struct F16Params {
+  int M, N;
+  int pairs_m, tiles_n, group_m, ksplit, nkb;   // nkb: stages of 64 of K in all
+  const uint32_t *amax_a, *amax_b;
+  const float *alpha_dev;
+  const float *bias;
+  float *C;
+  int64_t ldc;
+  int act, accumulate, vec_c;    // vec_c: C goes out by bulk tensor stores
+  int part_rows;                 // > 0: range r of K stores its bare sums to rows [r * part_rows, ...) behind maps.c
+  const float *target;
+  int64_t n_base;
+  float2 *stats;
+  float *target_logit;
+  const float *lse, *coef;
+  float *colsum_part;
+};
+
+// K-major tile [128 rows][64 k]: 128-byte rows, 128-byte swizzle, 8-row groups 1024 bytes apart.
+// MN-major tile: two boxes of [64 k][64 rows] 8192 bytes apart, 8-k-row groups 1024 bytes apart.
+template <bool MN>
+__device__ __forceinline__ uint64_t f16_desc(uint32_t addr) {
+  return MN ? smem_desc(addr, 8192, 1024, 2) : smem_desc(addr, 16, 1024, 2);
+}
+template <bool MN>
+__device__ __forceinline__ void f16_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int row0, int k0) {
+  if constexpr (MN) {
+    tma_load_2d_pair(dst, map, bar, row0, k0);
+    tma_load_2d_pair(dst + 8192u, map, bar, row0 + 64, k0);
+  } else {
+    tma_load_2d_pair(dst, map, bar, k0, row0);
+  }
+}
+
+// Column sums over a warp's 32 rows: v[j] of lane r is row r, column j; returns, in lane L, the sum of
+// column L. Halves the columns a lane is responsible for in each of five exchanges.
+__device__ __forceinline__ float warp_colsum32(float (&v)[32], int lane) {
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) {
+    const bool up = (lane & w) != 0;
+#pragma unroll
+    for (int i = 0; i < w; ++i) {
+      const float send = up ? v[i] : v[i + w], keep = up ? v[i + w] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, w);
+    }
+  }
+  return v[0];
+}
+
+// PROD: 3 = both operands are pairs, 2 = A is exact in its hi part.
+template <bool A_MN, bool B_MN, int PROD, int EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
+gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
+  constexpr int STAGES = PROD == 3 ? 3 : 4;
+  constexpr uint32_t A_BYTES = (PROD == 3 ? 2 : 1) * F16_TILE, STAGE_BYTES = A_BYTES + 2 * F16_TILE;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t smem_base = (smem_u32(smem) + 1023u) & ~1023u;
+  const uint32_t epi_base = smem_base + STAGES * STAGE_BYTES;
+  const uint32_t bars = epi_base + F16_EPI_WARPS * 4096u;
+  __shared__ uint32_t tmem_slot;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int num_pairs = (int)(gridDim.x >> 1), pair_id = (int)(blockIdx.x >> 1);
+  const int tiles_mn = p.pairs_m * p.tiles_n, num_items = tiles_mn * p.ksplit;
+  auto k_range = [&](int t, int &kb0, int &kb1) {      // (every range has at least one stage)
+    const int part = t / tiles_mn;
+    kb0 = (int)((int64_t)p.nkb * part / p.ksplit);
+    kb1 = (int)((int64_t)p.nkb * (part + 1) / p.ksplit);
+  };
+  // groups of group_m row pairs, the column tiles of a group one after the other: the pairs that run at
+  // the same time share a few bands of A and tiles of B in L2
+  auto tile_origin = [&](int w, int &m0, int &n0) {
+    const int t = w % tiles_mn;
+    const int group = t / (p.group_m * p.tiles_n);
+    const int gm0 = group * p.group_m;
+    const int gh = p.pairs_m - gm0 < p.group_m ? p.pairs_m - gm0 : p.group_m;
+    const int rem = t - group * (p.group_m * p.tiles_n);
+    m0 = (gm0 + rem % gh) * 256 + (int)rank * 128;
+    n0 = (rem / gh) * 256;
+  };
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (STAGES + s); };
+  auto acc_full = [&](int b) { return bars + 8u * (2 * STAGES + b); };
+  auto acc_empty = [&](int b) { return bars + 8u * (2 * STAGES + 2 + b); };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), 2 * F16_EPI_WARPS); }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = pair_id; t < num_items && ok; t += num_pairs) {
+        int m0, n0, kb, kb1;
+        tile_origin(t, m0, n0);
+        k_range(t, kb, kb1);
+        const int nh0 = n0 + (int)rank * 128;
+        for (; kb < kb1; ++kb, ++it) {
+          const int s = (int)(it % STAGES);
+          if (it >= STAGES && !mbar_wait(empty_bar(s), ((it / STAGES) - 1) & 1, 51)) { ok = false; break; }
+          const uint32_t st = smem_base + s * STAGE_BYTES, sb = st + A_BYTES;
+          if (leader) mbar_expect_tx(full_bar(s), 2 * STAGE_BYTES);   // both CTAs' bytes
+          const uint32_t fb = map_to_cta(full_bar(s), 0);
+          const int k0 = kb * F16_BK;
+          f16_load<A_MN>(st, &maps.a_hi, fb, m0, k0);
+          if constexpr (PROD == 3) f16_load<A_MN>(st + F16_TILE, &maps.a_lo, fb, m0, k0);
+          f16_load<B_MN>(sb, &maps.b_hi, fb, nh0, k0);
+          f16_load<B_MN>(sb + F16_TILE, &maps.b_lo, fb, nh0, k0);
+        }
+      }
+      if (!ok && leader) {
+        // copies in flight (of both CTAs) get a bounded chance to land before the pair exits
+        for (uint32_t j = it > STAGES ? it - STAGES : 0; j < it; ++j)
+          mbar_wait(full_bar((int)(j % STAGES)), (j / STAGES) & 1, 52);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      // fp32 accumulator, fp16 A and B (format 0), majors, N >> 3, M >> 4
+      const uint32_t idesc = (1u << 4) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
+                             ((uint32_t)(256 >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+      // 16 of K further: 32 bytes along a K-major row, 16 k-rows (2048 bytes) of an MN-major box
+      constexpr uint64_t A_STEP = A_MN ? 128 : 2, B_STEP = B_MN ? 128 : 2;
+      uint32_t j = 0;
+      bool ok = true;
+      for (int t = pair_id; t < num_items && ok; t += num_pairs) {
+        int kb, kb1;
+        k_range(t, kb, kb1);
+        for (; kb < kb1; ++kb, ++j) {
+          const int s = (int)(j % STAGES), b = (int)(j & 1);
+          if (j >= 2 && !mbar_wait_cluster(acc_empty(b), ((j >> 1) - 1) & 1, 53)) { ok = false; break; }
+          if (!mbar_wait(full_bar(s), (j / STAGES) & 1, 54)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t st = smem_base + s * STAGE_BYTES, sb = st + A_BYTES, d = tmem_base + 256u * b;
+          const uint64_t ah = f16_desc<A_MN>(st), bh = f16_desc<B_MN>(sb), bl = f16_desc<B_MN>(sb + F16_TILE);
+          if constexpr (PROD == 3) {
+            const uint64_t al = f16_desc<A_MN>(st + F16_TILE);
+#pragma unroll
+            for (int ks = 0; ks < F16_BK / 16; ++ks)
+              tc_mma_16bit_pair(d, al + ks * A_STEP, bh + ks * B_STEP, idesc, ks > 0);
+          }
+#pragma unroll
+          for (int ks = 0; ks < F16_BK / 16; ++ks)
+            tc_mma_16bit_pair(d, ah + ks * A_STEP, bl + ks * B_STEP, idesc, PROD == 3 || ks > 0);
+#pragma unroll
+          for (int ks = 0; ks < F16_BK / 16; ++ks)
+            tc_mma_16bit_pair(d, ah + ks * A_STEP, bh + ks * B_STEP, idesc, 1u);
+          tc_commit_pair(empty_bar(s));
+          tc_commit_pair(acc_full(b));
+        }
+      }
+    }
+  } else {
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t ebuf = epi_base + (uint32_t)(warp - 2) * 4096u;
+    const uint32_t row_addr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * 128);
+    const uint32_t empty_leader[2] = {map_to_cta(acc_empty(0), 0), map_to_cta(acc_empty(1), 0)};
+    const float f0 = half_unscale(p.amax_a);
+    const float f1 = half_unscale(p.amax_b) * (p.alpha_dev ? __ldg(p.alpha_dev) : 1.f);
+    uint32_t j = 0;
+    bool ok = true;
+    for (int t = pair_id; t < num_items && ok; t += num_pairs) {
+      int m0, n0, kb, kb1;
+      tile_origin(t, m0, n0);
+      k_range(t, kb, kb1);
+      float acc[128];
+#pragma unroll
+      for (int i = 0; i < 128; ++i) acc[i] = 0.f;
+      for (; kb < kb1; ++kb, ++j) {
+        const uint32_t b = j & 1;
+        if (!mbar_wait(acc_full((int)b), (j >> 1) & 1, 55)) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t r[32];
+          tc_ld32(row_addr + 256u * b + (uint32_t)(32 * c), r);
+          tc_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) acc[32 * c + i] += __uint_as_float(r[i]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(empty_leader[b]);
+      }
+      if (!ok) break;
+      const int nb = n0 + half * 128;            // this warp's first column
+      const int mq = m0 + q * 32, m = mq + lane; // its first row, this lane's row
+
+      if constexpr (EPI == F16_STORE) {
+        const bool parts = p.part_rows > 0;
+        const int row_off = parts ? (t / tiles_mn) * p.part_rows : 0;
+        const bool bulk = parts || p.vec_c;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int nc = nb + 32 * c;
+          if (nc < p.N && mq < p.M) {            // (uniform over the warp)
+            const float bv = (!parts && p.bias && nc + lane < p.N) ? __ldg(p.bias + nc + lane) : 0.f;
+            if (bulk) {                          // the previous chunk's store has read the buffer
+              if (lane == 0) bulk_wait_read0();
+              __syncwarp();
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              float4 v = make_float4(acc[32 * c + 4 * u], acc[32 * c + 4 * u + 1], acc[32 * c + 4 * u + 2], acc[32 * c + 4 * u + 3]);
+              if (!parts) {
+                v.x = (v.x * f0) * f1; v.y = (v.y * f0) * f1; v.z = (v.z * f0) * f1; v.w = (v.w * f0) * f1;
+              }
+              sts128(ebuf + (uint32_t)lane * 128u + (uint32_t)((u ^ (lane & 7)) * 16), v);
+            }
+            __syncwarp();
+            if (!parts && (p.bias || p.act || !bulk)) {
+              // lanes along the row: bias and activation, and the stores where C has no 16-byte rows
+              const uint32_t col = (uint32_t)(lane >> 2), sub = (uint32_t)(lane & 3) * 4u;
+#pragma unroll 4
+              for (int r = 0; r < 32; ++r) {
+                const uint32_t a = ebuf + (uint32_t)r * 128u + ((col ^ (uint32_t)(r & 7)) * 16u) + sub;
+                float v;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+                v += bv;
+                if (p.act) v = act_fwd(p.act, v);
+                if (bulk) {
+                  asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
+                } else if (mq + r < p.M && nc + lane < p.N) {
+                  float *cp = p.C + (int64_t)(mq + r) * p.ldc + nc + lane;
+                  *cp = p.accumulate ? *cp + v : v;
+                }
+              }
+            }
+            if (bulk) {
+              fence_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                if (p.accumulate && !parts) tma_reduce_add_2d(&maps.c, ebuf, nc, mq);
+                else tma_store_2d(&maps.c, ebuf, nc, mq + row_off);
+                bulk_commit();
+              }
+            } else {
+              __syncwarp();
+            }
+          }
+        }
+      } else {
+        const bool row_ok = m < p.M;
+        const float tg = row_ok ? __ldg(p.target + m) : -1.f;
+        const int64_t v0 = p.n_base + nb;
+        // this lane's target among the warp's 128 columns, or a number that no column has
+        const int tl = (tg >= (float)v0 && tg < (float)(v0 + 128)) ? (int)((int64_t)tg - v0) : -1;
+        float bv[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) bv[c] = (p.bias && nb + 32 * c + lane < p.N) ? __ldg(p.bias + nb + 32 * c + lane) : 0.f;
+        const bool has_bias = p.bias != nullptr;
+#pragma unroll
+        for (int i = 0; i < 128; ++i) {
+          acc[i] = (acc[i] * f0) * f1;
+          if (has_bias) acc[i] += __shfl_sync(0xffffffffu, bv[i >> 5], i & 31);
+        }
+        if constexpr (EPI == F16_STATS) {
+          // the sum of 128 exponentials below a maximum of their own; -inf columns (banned classes) add 0
+          float mx = -INFINITY, tv = 0.f;
+          bool nan = false;
+#pragma unroll
+          for (int i = 0; i < 128; ++i) {
+            if (nb + i >= p.N) acc[i] = -INFINITY;
+            nan |= acc[i] != acc[i];
+            mx = fmaxf(mx, acc[i]);
+            if (i == tl) tv = acc[i];
+          }
+          float sum = 0.f;
+          if (mx > -INFINITY) {
+#pragma unroll
+            for (int i = 0; i < 128; ++i) sum += __expf(acc[i] - mx);
+          }
+          if (nan) sum = NAN;
+          if (row_ok) {
+            p.stats[(v0 >> 7) * (int64_t)p.M + m] = make_float2(mx, sum);
+            if (tl >= 0) p.target_logit[m] = tv;
+          }
+        } else {
+          const float lse = row_ok ? __ldg(p.lse + m) : 0.f, cf = row_ok ? __ldg(p.coef + m) : 0.f;
+          const bool dead = cf == 0.f;     // a row that is left out: exactly zero, whatever its logits are
+#pragma unroll
+          for (int i = 0; i < 128; ++i) {
+            const float e = expf(acc[i] - lse) - (i == tl ? 1.f : 0.f);
+            acc[i] = dead ? 0.f : e * cf;
+          }
+          // hi and lo of two chunks of 64 columns through the warp's buffer
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            if (nb + 64 * c < p.N && mq < p.M) {
+#pragma unroll
+              for (int part = 0; part < 2; ++part) {
+                if (lane == 0) bulk_wait_read0();
+                __syncwarp();
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                  uint32_t w[4];
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    const float x0 = acc[64 * c + 8 * u + 2 * k] * F16_D_SCALE, x1 = acc[64 * c + 8 * u + 2 * k + 1] * F16_D_SCALE;
+                    __half2 h = __floats2half2_rn(x0, x1);
+                    if (part) {
+                      const float2 hf = __half22float2(h);
+                      h = __floats2half2_rn(x0 - hf.x, x1 - hf.y);
+                    }
+                    w[k] = *reinterpret_cast<uint32_t *>(&h);
+                  }
+                  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                               ::"r"(ebuf + (uint32_t)lane * 128u + (uint32_t)((u ^ (lane & 7)) * 16)),
+                               "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                  tma_store_2d(part ? &maps.d_lo : &maps.d_hi, ebuf, nb + 64 * c, mq);
+                  bulk_commit();
+                }
+              }
+            }
+          }
+          if (p.colsum_part && mq < p.M) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              float v[32];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = acc[32 * c + i];
+              const float s = warp_colsum32(v, lane);
+              if (nb + 32 * c + lane < p.N) p.colsum_part[(int64_t)(mq >> 5) * p.N + nb + 32 * c + lane] = s;
+            }
+          }
+        }
+      }
+    }
+    if (lane == 0) bulk_wait0();   // the stores have left shared memory and are complete
+  }
+  tc_fence_before();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+  }
+}
+
+// C = act(sum over the ranges of K, in order, unscaled, + bias), or C += it.
+__global__ void __launch_bounds__(256)
+gemm_f16_finish_kernel(const F16Params p, const float *__restrict__ partial, int64_t ld_partial, int64_t slice, int parts) {
+  const float f0 = half_unscale(p.amax_a);
+  const float f1 = half_unscale(p.amax_b) * (p.alpha_dev ? __ldg(p.alpha_dev) : 1.f);
+  const int n = (int)(blockIdx.x * blockDim.x + threadIdx.x);
+  if (n >= p.N) return;
+  const float bv = p.bias ? __ldg(p.bias + n) : 0.f;
+  for (int m = (int)blockIdx.y; m < p.M; m += (int)gridDim.y) {
+    const float *src = partial + (int64_t)m * ld_partial + n;
+    float v = 0.f;
+    for (int s0 = 0; s0 < parts; s0 += 8) {
+      float t[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) t[u] = s0 + u < parts ? __ldcs(src + (int64_t)(s0 + u) * slice) : 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v += t[u];
+    }
+    v = (v * f0) * f1 + bv;
+    if (p.act) v = act_fwd(p.act, v);
+    float *c = p.C + (int64_t)m * p.ldc + n;
+    *c = p.accumulate ? *c + v : v;
+  }
+}
+
+// ---------------------------------------------------------------------------- passes over fp32 arrays
+// Eight consecutive columns per thread; VEC: 128-bit loads (leading dimension and base allow them).
+template <bool VEC>
+__device__ __forceinline__ void load8(const float *src, int64_t left, float (&v)[8]) {
+  if (VEC && left >= 8) {
+    const float4 a = __ldg(reinterpret_cast<const float4 *>(src)), b = __ldg(reinterpret_cast<const float4 *>(src) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? __ldg(src + i) : 0.f;
+  }
+}
+__device__ __forceinline__ void row_and_col(int64_t i, int64_t per_row, bool narrow, int64_t &r, int64_t &c) {
+  r = narrow ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row;
+  c = i - r * per_row;
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(256)
+amax_kernel(const float *__restrict__ x, int64_t rows, int64_t cols, int64_t ld, const float *__restrict__ target,
+            uint32_t *__restrict__ amax) {
+  const int64_t per_row = (cols + 7) / 8, total = rows * per_row, step = (int64_t)gridDim.x * blockDim.x;
+  const bool narrow = total < ((int64_t)1 << 31);
+  uint32_t best = 0;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
+    int64_t r, c;
+    row_and_col(i, per_row, narrow, r, c);
+    if (target && __ldg(target + r) < 0.f) continue;
+    float v[8];
+    load8<VEC>(x + r * ld + c * 8, cols - c * 8, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t b = __float_as_uint(v[k]) & 0x7FFFFFFFu;
+      if (b < 0x7F800000u && b > best) best = b;
+    }
+  }
+  best = __reduce_max_sync(0xffffffffu, best);
+  if ((threadIdx.x & 31) == 0 && best) atomicMax(amax, best);   // (a maximum: any order gives the same bits)
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(256)
+half_split_kernel(const float *__restrict__ x, int64_t rows, int64_t cols, int64_t ld, const float *__restrict__ target,
+                  const uint32_t *__restrict__ amax, __half *__restrict__ hi, __half *__restrict__ lo, int64_t ld_out) {
+  const int64_t per_row = (cols + 7) / 8, total = rows * per_row, step = (int64_t)gridDim.x * blockDim.x;
+  const bool narrow = total < ((int64_t)1 << 31);
+  const float s = half_scale(amax);
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
+    int64_t r, c;
+    row_and_col(i, per_row, narrow, r, c);
+    float v[8];
+    if (target && __ldg(target + r) < 0.f) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = 0.f;
+    } else {
+      load8<VEC>(x + r * ld + c * 8, cols - c * 8, v);
+    }
+    __half h[8], l[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) half_pair(v[k] * s, h[k], l[k]);
+    *reinterpret_cast<uint4 *>(hi + r * ld_out + c * 8) = *reinterpret_cast<uint4 *>(h);   // (ld_out covers whole groups of 8)
+    *reinterpret_cast<uint4 *>(lo + r * ld_out + c * 8) = *reinterpret_cast<uint4 *>(l);
+  }
+}
+
+static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int launch_amax(const float *x, int64_t rows, int64_t cols, int64_t ld, const float *target, uint32_t *amax,
+                cudaStream_t s) {
+  if (rows <= 0 || cols <= 0) return ENDIA_B200_OK;
+  if (!target && ld == cols) { cols *= rows; ld = cols; rows = 1; }
+  const int grid = grid_for(rows * ceil_div(cols, 8), 256, 8);
+  if (aligned16(x) && (ld % 4 == 0 || rows == 1)) amax_kernel<true><<<grid, 256, 0, s>>>(x, rows, cols, ld, target, amax);
+  else amax_kernel<false><<<grid, 256, 0, s>>>(x, rows, cols, ld, target, amax);
+  EB_LAUNCH_CHECK();
+  return ENDIA_B200_OK;
+}
+
+int launch_half_split(const float *x, int64_t rows, int64_t cols, int64_t ld, const float *target,
+                      const uint32_t *amax, __half *hi, __half *lo, int64_t ld_out, cudaStream_t s) {
+  if (rows <= 0 || cols <= 0) return ENDIA_B200_OK;
+  const int grid = grid_for(rows * ceil_div(cols, 8), 256, 8);
+  if (aligned16(x) && (ld % 4 == 0 || rows == 1)) half_split_kernel<true><<<grid, 256, 0, s>>>(x, rows, cols, ld, target, amax, hi, lo, ld_out);
+  else half_split_kernel<false><<<grid, 256, 0, s>>>(x, rows, cols, ld, target, amax, hi, lo, ld_out);
+  EB_LAUNCH_CHECK();
+  return ENDIA_B200_OK;
+}
+
+// ---------------------------------------------------------------------------------------- host side
+// Tensor map of a row-major [outer, inner] array: fp16 boxes with the 128-byte swizzle (64 elements
+// wide) for operands and d, fp32 boxes of [32][32] for C. Elements outside read as zero and are not written.
+static int make_map_16(CUtensorMap *map, const void *base, int64_t inner, int64_t outer, int64_t ld, int box_outer) {
+  cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer}, strides[1] = {(cuuint64_t)ld * 2};
+  cuuint32_t box[2] = {64u, (cuuint32_t)box_outer}, estr[2] = {1u, 1u};
+  const CUresult r = encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(base), dims, strides, box, estr,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  EB_REQUIRE(r == CUDA_SUCCESS, ENDIA_B200_ECUDA, "fp16-pair product: cuTensorMapEncodeTiled failed with code %d", (int)r);
+  return ENDIA_B200_OK;
+}
+static int make_map_32(CUtensorMap *map, const void *base, int64_t inner, int64_t outer, int64_t ld) {
+  cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer}, strides[1] = {(cuuint64_t)ld * 4};
+  cuuint32_t box[2] = {32u, 32u}, estr[2] = {1u, 1u};
+  const CUresult r = encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void *>(base), dims, strides, box, estr,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  EB_REQUIRE(r == CUDA_SUCCESS, ENDIA_B200_ECUDA, "fp16-pair product: cuTensorMapEncodeTiled (C) failed with code %d", (int)r);
+  return ENDIA_B200_OK;
+}
+
+bool gemm_f16_available() { return encode_fn() != nullptr; }
+
+// Ranges of K of an F16_STORE product: when its tiles leave half of the CTA pairs idle, each tile's
+// reduction is cut into up to 16 ranges of at least 512.
+static int k_ranges(int64_t M, int64_t N, int64_t K) {
+  const int64_t tiles = ceil_div(M, 256) * ceil_div(N, 256), cap = (sm_count() > 0 ? sm_count() : 148) / 2;
+  if (2 * tiles > cap) return 1;
+  int64_t sp = cap / tiles;
+  if (sp > K / 512) sp = K / 512;
+  if (sp > 16) sp = 16;
+  return sp >= 2 ? (int)sp : 1;
+}
+size_t gemm_f16_partial_bytes(int64_t M, int64_t N, int64_t K) {
+  const int sp = k_ranges(M, N, K);
+  return sp < 2 ? 0 : sizeof(float) * (size_t)sp * (size_t)(ceil_div(M, 256) * 256) * (size_t)(ceil_div(N, 4) * 4);
+}
+
+template <bool A_MN, bool B_MN, int PROD, int EPI>
+static int launch_kernel(const F16Maps &maps, const F16Params &p, cudaStream_t s) {
+  constexpr int STAGES = PROD == 3 ? 3 : 4;
+  constexpr size_t SMEM = (size_t)STAGES * ((PROD == 3 ? 4 : 3) * F16_TILE) + F16_EPI_WARPS * 4096 + 1024 + 256;
+  auto kern = gemm_f16_kernel<A_MN, B_MN, PROD, EPI>;
+  static int max_pairs = 0;
+  if (!max_pairs) {
+    EB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2);
+    cfg.blockDim = dim3(320);
+    cfg.dynamicSmemBytes = SMEM;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = 2; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    int nc = 0;
+    if (cudaOccupancyMaxActiveClusters(&nc, kern, &cfg) != cudaSuccess || nc <= 0) {
+      cudaGetLastError();
+      nc = (sm_count() > 0 ? sm_count() : 148) / 2;
+    }
+    max_pairs = nc;
+  }
+  const int items = p.pairs_m * p.tiles_n * p.ksplit, pairs = items < max_pairs ? items : max_pairs;
+  kern<<<dim3((unsigned)(2 * pairs)), 320, SMEM, s>>>(maps, p);
+  EB_LAUNCH_CHECK();
+  return ENDIA_B200_OK;
+}
+
+int launch_gemm_f16(const F16Gemm &g, bool a_mn, bool b_mn, int epilogue, cudaStream_t s) {
+  EB_REQUIRE(gemm_f16_available(), ENDIA_B200_ECUDA, "fp16-pair product: the driver has no cuTensorMapEncodeTiled");
+  EB_REQUIRE(g.M >= 1 && g.N >= 1 && g.K >= 1 && g.M <= (1 << 30) && g.N <= (1 << 30) && g.K <= (1 << 30),
+             ENDIA_B200_ELIMIT, "fp16-pair product: sizes must lie in [1, 2^30]");
+  F16Maps maps;
+  F16Params p{};
+  int st;
+  const int64_t a_in = a_mn ? g.M : g.K, a_out = a_mn ? g.K : g.M, b_in = b_mn ? g.N : g.K, b_out = b_mn ? g.K : g.N;
+  const int a_box = a_mn ? F16_BK : 128, b_box = b_mn ? F16_BK : 128;
+  const bool exact_a = g.a.lo == nullptr;
+  if ((st = make_map_16(&maps.a_hi, g.a.hi, a_in, a_out, g.a.ld, a_box))) return st;
+  if ((st = make_map_16(&maps.a_lo, exact_a ? g.a.hi : g.a.lo, a_in, a_out, g.a.ld, a_box))) return st;
+  if ((st = make_map_16(&maps.b_hi, g.b.hi, b_in, b_out, g.b.ld, b_box))) return st;
+  if ((st = make_map_16(&maps.b_lo, g.b.lo, b_in, b_out, g.b.ld, b_box))) return st;
+  maps.c = maps.d_hi = maps.d_lo = maps.a_hi;
+  p.M = (int)g.M; p.N = (int)g.N;
+  p.pairs_m = (int)ceil_div(g.M, 256); p.tiles_n = (int)ceil_div(g.N, 256);
+  p.group_m = 8;
+  p.nkb = (int)ceil_div(g.K, F16_BK);
+  p.ksplit = 1;
+  p.amax_a = g.a.amax; p.amax_b = g.b.amax; p.alpha_dev = g.alpha_dev; p.bias = g.bias;
+  p.C = g.C; p.ldc = g.ldc; p.act = g.act; p.accumulate = g.accumulate ? 1 : 0;
+  p.target = g.target; p.n_base = g.n_base; p.stats = g.stats; p.target_logit = g.target_logit;
+  p.lse = g.lse; p.coef = g.coef; p.colsum_part = g.colsum_part;
+  EB_REQUIRE((int64_t)p.pairs_m * p.tiles_n <= (1 << 26), ENDIA_B200_ELIMIT, "fp16-pair product: too many tiles");
+  if (epilogue == F16_STATS) {
+    if (!a_mn && b_mn && !exact_a) return launch_kernel<false, true, 3, F16_STATS>(maps, p, s);
+  } else if (epilogue == F16_DLOGITS) {
+    if ((st = make_map_16(&maps.d_hi, g.d_hi, g.N, g.M, g.ld_d, 32))) return st;
+    if ((st = make_map_16(&maps.d_lo, g.d_lo, g.N, g.M, g.ld_d, 32))) return st;
+    if (!a_mn && b_mn && !exact_a) return launch_kernel<false, true, 3, F16_DLOGITS>(maps, p, s);
+  } else {
+    const int sp = g.partial ? k_ranges(g.M, g.N, g.K) : 1;
+    const int64_t ldp = ceil_div(g.N, 4) * 4;
+    p.vec_c = aligned16(g.C) && g.ldc % 4 == 0;
+    if (sp > 1) {
+      p.ksplit = sp;
+      p.part_rows = p.pairs_m * 256;
+      if ((st = make_map_32(&maps.c, g.partial, g.N, (int64_t)sp * p.part_rows, ldp))) return st;
+    } else if (p.vec_c) {
+      if ((st = make_map_32(&maps.c, g.C, g.N, g.M, g.ldc))) return st;
+    }
+    if (!a_mn && b_mn && !exact_a) st = launch_kernel<false, true, 3, F16_STORE>(maps, p, s);
+    else if (!a_mn && !b_mn && !exact_a) st = launch_kernel<false, false, 3, F16_STORE>(maps, p, s);
+    else if (a_mn && b_mn && !exact_a) st = launch_kernel<true, true, 3, F16_STORE>(maps, p, s);
+    else if (a_mn && b_mn) st = launch_kernel<true, true, 2, F16_STORE>(maps, p, s);
+    else { set_error("fp16-pair product: no kernel for these layouts"); return ENDIA_B200_EINVAL; }
+    if (st || sp < 2) return st;
+    const dim3 grid((unsigned)ceil_div(g.N, 256), (unsigned)(g.M < 1024 ? g.M : 1024));
+    gemm_f16_finish_kernel<<<grid, 256, 0, s>>>(p, g.partial, ldp, (int64_t)p.part_rows * ldp, sp);
+    EB_LAUNCH_CHECK();
+    return ENDIA_B200_OK;
+  }
+  set_error("fp16-pair product: no kernel for these layouts");
+  return ENDIA_B200_EINVAL;
+}
+
+int gemm_fp32(int ta, int tb, int64_t M, int64_t N, int64_t K, const float *A, int64_t lda, const float *B, int64_t ldb,
+              float *C, int64_t ldc, const float *bias, int act, float beta, cudaStream_t s) {
+  GemmParams p{};
+  p.A = A; p.B = B; p.C = C; p.M = M; p.N = N; p.K = K; p.lda = lda; p.ldb = ldb; p.ldc = ldc;
+  p.vec_a = aligned16(A) && lda % 4 == 0;
+  p.vec_b = aligned16(B) && ldb % 4 == 0;
+  p.vec_c = aligned16(C) && ldc % 4 == 0;
+  p.epi.alpha = 1.f; p.epi.beta = beta; p.epi.bias = bias; p.epi.act = act;
+  if (skinny_gemm_supported(p, tb, 1)) return launch_gemm_skinny(p, ta, tb, s);
+  return launch_gemm_ffma(p, ta, tb, 1, s);
+}
+
+int f16_status_and_clear(cudaStream_t s) {
+  int h = 0;
+  if (cudaStreamSynchronize(s) != cudaSuccess) return -1;
+  if (cudaMemcpyFromSymbol(&h, g_tc_status, sizeof(int)) != cudaSuccess) return -1;
+  if (h) {
+    int z = 0;
+    cudaMemcpyToSymbol(g_tc_status, &z, sizeof(int));
+  }
+  return h;
+}
+
+}  // namespace eb

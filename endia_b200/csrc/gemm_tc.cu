@@ -29,7 +29,7 @@
 // (endia_b200_device_status) and the CTA drains and returns.
 #include "common.cuh"
 #include "gemm.cuh"
-#include <cuda.h>
+#include "tc_ptx.cuh"
 #include <cuda_bf16.h>
 #include <stdlib.h>
 
@@ -37,38 +37,7 @@ namespace eb {
 
 constexpr int TC_BM = 128;
 constexpr int TC_GROUP_M = 8;
-constexpr uint32_t TC_WAIT_LIMIT = 1u << 22;
 
-static __device__ int g_tc_status = 0;    // 0 ok, else the code of the first wait that gave up
-
-
-// ------------------------------------------------------------------------------- PTX helpers
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-  return (uint32_t)__cvta_generic_to_shared(p);
-}
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-  return ok != 0;
-}
-// Bounded wait: false (and the status flag set) when the phase never completes.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int code,
-                                          uint32_t limit = TC_WAIT_LIMIT) {
-  for (uint32_t it = 0; it < limit; ++it)
-    if (mbar_try_wait(bar, parity)) return true;
-  atomicCAS(&g_tc_status, 0, code);
-  return false;
-}
 
 // Self-test of the give-up path: one thread waits, with the wait above and a limit of `polls`, on a
 // barrier that nothing ever arrives at. The wait runs out, records code 99 and the kernel returns.
@@ -79,60 +48,6 @@ __global__ void wait_selftest_kernel(uint32_t polls) {
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     mbar_wait(smem_u32(&bar), 0, 99, polls);
   }
-}
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar,
-                                            int c0, int c1) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-      ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void tc_mma_tf32(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                                            uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
-}
-__device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
-        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
-        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
-        "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr) : "memory");
-}
-__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr) : "memory");
-}
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
-// Shared-memory matrix descriptor (descriptor version 1): start address, leading and stride byte
-// offsets in 16-byte units, and the swizzle mode: 2 = 128-byte swizzle in 16-byte units (K-major
-// tiles), 1 = 128-byte swizzle in 32-byte units, the only mode MN-major 32-bit operands accept.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo_bytes, uint32_t sbo_bytes,
-                                              uint32_t layout_type) {
-  uint64_t d = 0;
-  d |= (uint64_t)((addr & 0x3FFFFu) >> 4);
-  d |= (uint64_t)((lbo_bytes >> 4) & 0x3FFFu) << 16;
-  d |= (uint64_t)((sbo_bytes >> 4) & 0x3FFFu) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)layout_type << 61;
-  return d;
 }
 // K-major tile: rows of BK floats (128 bytes with the 128-byte swizzle, 64 with the 64-byte one),
 // 8-row groups contiguous. MN-major tile: boxes of [BK k][32 rows] (BK*128 bytes apart), inside
@@ -149,30 +64,6 @@ struct TcMaps {
   CUtensorMap c;   // output, boxes of [32 rows][32 floats] (persistent kernel, when C allows 128-bit access)
 };
 
-// Bulk tensor store of one [32 rows][128 bytes] shared-memory box (128-byte swizzle) to C at
-// column x, row y; rows and columns beyond the array are clipped by the copy engine.
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, uint32_t src, int x, int y) {
-  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
-               ::"l"(map), "r"(src), "r"(x), "r"(y) : "memory");
-}
-// The same box added (fp32) to what C holds.
-__device__ __forceinline__ void tma_reduce_add_2d(const CUtensorMap *map, uint32_t src, int x, int y) {
-  asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];"
-               ::"l"(map), "r"(src), "r"(x), "r"(y) : "memory");
-}
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read0() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait0() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-__device__ __forceinline__ float4 lds128(uint32_t a) {
-  float4 v;
-  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ void sts128(uint32_t a, float4 v) {
-  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
-}
 
 // The fused epilogue on four consecutive columns n..n+3 of row m; `vec` says that the bias, the
 // activation-derivative source and C may be read with 128-bit loads at this position.
@@ -427,31 +318,6 @@ gemm_tc_kernel(const __grid_constant__ TcMaps maps, const GemmParams p, int tile
 // memory, the resource that bounds the one-CTA kernel. Loads of both CTAs signal the leader's
 // "full" barriers; the leader's commits are multicast to both CTAs' "empty" and accumulator
 // barriers. No load is multicast.
-__device__ __forceinline__ uint32_t cluster_ctarank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t map_to_cta(uint32_t smem_addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// Tile load whose completion bytes are counted on a barrier of the pair's leader CTA.
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap *map, uint32_t leader_bar,
-                                                 int c0, int c1) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-      ::"r"(dst), "l"(map), "r"(leader_bar), "r"(c0), "r"(c1) : "memory");
-}
-__device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-      ::"r"(bar), "h"((uint16_t)3) : "memory");
-}
 __device__ __forceinline__ void tc_mma_tf32_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
                                                  uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -461,14 +327,6 @@ __device__ __forceinline__ void tc_mma_tf32_pair(uint32_t d_tmem, uint64_t a_des
       ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-__device__ __forceinline__ void tc_mma_bf16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                                                 uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
-}
 // bf16 tiles of 32 k: K-major rows of 64 bytes (64-byte swizzle, 8-row groups 512 bytes apart);
 // MN-major boxes of [32 k][64 rows] (128 bytes per k-row, 128-byte swizzle, 8 k-rows per atom,
 // boxes 4096 bytes apart).
@@ -691,23 +549,6 @@ __device__ __forceinline__ void tc_epilogue_warp_bulk(const uint32_t (&v1)[32], 
 // fused epilogue and the stores of a tile run beside the products of the next one. What is saved per
 // tile: the CTA launch, the tensor-memory allocation, the barrier set-up and the empty pipeline.
 // The epilogue warps have 4 KB of shared memory each of their own (the stages are never free).
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
-}
-// Bounded wait that acquires at cluster scope (the arrivals come from both CTAs of the pair).
-__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, int code) {
-  for (uint32_t it = 0; it < TC_WAIT_LIMIT; ++it) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    if (ok) return true;
-  }
-  atomicCAS(&g_tc_status, 0, code);
-  return false;
-}
 
 // SCHEME 0: 3xTF32, the stage holds the fp32 tile and its fp32 low part of each operand.
 // SCHEME 1: the stage holds the fp32 tile (tf32 MMA hi*hi into the main accumulator) and two bf16
@@ -902,8 +743,8 @@ gemm_tc2p_kernel(const __grid_constant__ TcMaps maps, const GemmParams p, int pa
 #pragma unroll
             for (int ks = 0; ks < BK / 16; ++ks) {
               const uint32_t acc = (run | kl | ks) ? 1u : 0u;   // (runs on over the runs of a work item)
-              tc_mma_bf16_pair(tmem_base + BN, a16l + ks * A16_STEP, b16h + ks * B16_STEP, idesc16, acc);
-              tc_mma_bf16_pair(tmem_base + BN, a16h + ks * A16_STEP, b16l + ks * B16_STEP, idesc16, 1u);
+              tc_mma_16bit_pair(tmem_base + BN, a16l + ks * A16_STEP, b16h + ks * B16_STEP, idesc16, acc);
+              tc_mma_16bit_pair(tmem_base + BN, a16h + ks * A16_STEP, b16l + ks * B16_STEP, idesc16, 1u);
             }
 #pragma unroll
             for (int ks = 0; ks < BK / 8; ++ks)
@@ -1088,12 +929,7 @@ int tc_default_scheme() {
 }
 
 // ---------------------------------------------------------------------------------- host side
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
-                                  const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
-                                  const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
+EncodeTiledFn encode_fn() {
   static EncodeTiledFn fn = nullptr;
   static bool tried = false;
   if (!tried) {
@@ -1453,6 +1289,8 @@ int launch_gemm_tc(const GemmParams &p_in, int trans_a, int trans_b, cudaStream_
   return st;
 }
 
+int f16_status_and_clear(cudaStream_t s);      // the same for gemm_f16.cu's kernels
+
 int tc_status_and_clear(cudaStream_t s) {
   int h = 0;
   if (cudaStreamSynchronize(s) != cudaSuccess) return -1;
@@ -1482,6 +1320,8 @@ extern "C" int endia_b200_device_status(void *stream) {
   int st = eb::require_device();
   if (st) return st;
   int code = eb::tc_status_and_clear(eb::as_stream(stream));
+  const int code16 = eb::f16_status_and_clear(eb::as_stream(stream));
+  if (code == 0) code = code16;
   if (code < 0) {
     eb::set_error("device_status: synchronising the stream failed: %s", cudaGetErrorString(cudaGetLastError()));
     return ENDIA_B200_ECUDA;

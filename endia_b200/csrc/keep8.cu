@@ -1,0 +1,434 @@
+// Activations held in 8 bits for the backward pass, and the linear layer that uses them.
+//
+// Form: per row, blocks of 32 consecutive features share a power-of-two scale:
+//   x ~ q * 2^e,  e the smallest integer with round(max|x| / 2^e) <= 127,  q = round(x / 2^e) in [-127, 127]
+// (round half to even; e >= -126). 8.25 bits per value, an error of at most half of 2^e, which is between
+// max/127.5/2 and max/63.75/2. With keep_sign a value that is not zero gets |q| >= 1, so that the
+// derivative of a ReLU taken from its kept output is the exact one. An infinite or NaN value is kept as
+// q = -128 and reads back as NaN; it does not count in the block's maximum.
+// Why a power of two: x / 2^e and q * 2^e are exact in fp32, and q * 2^e is exact in fp16 after one scale
+// for the whole array, so the weight gradient h^T ds needs two fp16 products instead of three.
+// Layout: a head of 256 bytes ([0]: bits of the largest finite |x|), q [rows][cols rounded up to 32],
+// e + 127 [rows][cols / 32 rounded up] as bytes.
+//
+// The layer: out = act(x W + b) from x itself; for its backward pass only the kept forms are read:
+//   ds = g act'(out),  dx = ds W^T,  dW = x8^T ds,  db = sum over the rows of ds.
+// Replaces, for such a layer, the products of matmul_vjp and the masks of relu/tanh/sigmoid
+// (endia/functional/binary_ops/matmul_op.mojo:278-284, relu_op.mojo:95, tanh_op.mojo:92, sigmoid_op.mojo:98).
+#include "gemm_f16.cuh"
+#include "gemm.cuh"
+
+using namespace eb;
+
+namespace eb {
+
+struct Kept {
+  uint32_t *amax;
+  int8_t *q;
+  uint8_t *e;
+  int64_t ldq, lde;
+};
+__host__ __device__ static inline Kept kept_view(void *p, int64_t rows, int64_t cols) {
+  Kept k;
+  char *c = static_cast<char *>(p);
+  k.ldq = (cols + 31) / 32 * 32;
+  k.lde = k.ldq / 32;
+  k.amax = reinterpret_cast<uint32_t *>(c);
+  k.q = reinterpret_cast<int8_t *>(c + 256);
+  k.e = reinterpret_cast<uint8_t *>(c + 256 + rows * k.ldq);
+  return k;
+}
+
+// 8 lanes per block of 32, four values each (128-bit loads where VEC).
+template <bool VEC>
+__global__ void __launch_bounds__(256)
+keep8_kernel(const float *__restrict__ x, int64_t ld, int64_t rows, int64_t cols, int keep_sign, Kept k) {
+  const int64_t per_row = k.ldq / 4, total = rows * per_row, step = (int64_t)gridDim.x * blockDim.x;
+  const bool narrow = total < ((int64_t)1 << 31);
+  uint32_t best = 0;
+  // (whole warps take part in the exchanges: total is a multiple of 8, the tail of a warp idles along)
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i - (threadIdx.x & 31) < total; i += step) {
+    const bool in = i < total;
+    const int64_t r = !in ? 0 : (narrow ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row);
+    const int64_t c = in ? (i - r * per_row) * 4 : 0, left = in ? cols - c : 0;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    const float *src = x + r * ld + c;
+    if (VEC && left >= 4) {
+      const float4 t = __ldg(reinterpret_cast<const float4 *>(src));
+      v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) if (u < left) v[u] = __ldg(src + u);
+    }
+    uint32_t mx = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t b = __float_as_uint(v[u]) & 0x7FFFFFFFu;
+      if (b < 0x7F800000u && b > mx) mx = b;
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+      const uint32_t b = __shfl_xor_sync(0xffffffffu, mx, o);
+      mx = b > mx ? b : mx;
+    }
+    best = mx > best ? mx : best;
+    // max / 2^e < 127.5: 127.5 = 64 * 1.9921875
+    int e = (int)(mx >> 23) - 127 - 6 + ((mx & 0x7FFFFFu) >= 0x7F0000u ? 1 : 0);
+    e = e < -126 ? -126 : e;
+    const float down = pow2f_exact(-e);
+    char4 q;
+    int8_t *qp = reinterpret_cast<int8_t *>(&q);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t b = __float_as_uint(v[u]) & 0x7FFFFFFFu;
+      int n = b < 0x7F800000u ? __float2int_rn(v[u] * down) : -128;
+      if (keep_sign && n == 0 && b != 0) n = v[u] < 0.f ? -1 : 1;
+      qp[u] = (int8_t)n;
+    }
+    if (in) {
+      *reinterpret_cast<char4 *>(k.q + r * k.ldq + c) = q;
+      if ((threadIdx.x & 7) == 0) k.e[r * k.lde + c / 32] = (uint8_t)(e + 127);
+    }
+  }
+  best = __reduce_max_sync(0xffffffffu, best);
+  if ((threadIdx.x & 31) == 0 && best) atomicMax(k.amax, best);
+}
+
+// Eight consecutive kept values of row r from column c (a multiple of 8), times `s`.
+__device__ __forceinline__ void kept8(const Kept &k, int64_t r, int64_t c, float s, float (&v)[8]) {
+  const uint2 w = __ldg(reinterpret_cast<const uint2 *>(k.q + r * k.ldq + c));
+  const float unit = pow2f_exact((int)__ldg(k.e + r * k.lde + c / 32) - 127);
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const int n = (int)(int8_t)(((u < 4 ? w.x : w.y) >> (8 * (u & 3))) & 0xFFu);
+    v[u] = n == -128 ? NAN : ((float)n * unit) * s;
+  }
+}
+
+__global__ void __launch_bounds__(256)
+kept_read_kernel(Kept k, int64_t rows, int64_t cols, float *__restrict__ out) {
+  const int64_t per_row = k.ldq / 8, total = rows * per_row, step = (int64_t)gridDim.x * blockDim.x;
+  const bool vec = cols % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
+    const int64_t r = i / per_row, c = (i - r * per_row) * 8;
+    float v[8];
+    kept8(k, r, c, 1.f, v);
+    float *dst = out + r * cols + c;
+    if (vec && c + 8 <= cols) {
+      reinterpret_cast<float4 *>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4 *>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) if (c + u < cols) dst[u] = v[u];
+    }
+  }
+}
+
+// The kept values as one fp16 operand (exact: q has 7 bits; values below 2^-24 of the array's scale
+// step, 2^-38 of its largest value, round to nothing).
+__global__ void __launch_bounds__(256)
+kept_half_kernel(Kept k, int64_t rows, __half *__restrict__ out) {
+  const int64_t per_row = k.ldq / 8, total = rows * per_row, step = (int64_t)gridDim.x * blockDim.x;
+  const bool narrow = total < ((int64_t)1 << 31);
+  const float s = half_scale(k.amax);
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
+    const int64_t r = narrow ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row, c = (i - r * per_row) * 8;
+    float v[8];
+    kept8(k, r, c, s, v);
+    __half h[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) h[u] = __float2half_rn(v[u]);
+    *reinterpret_cast<uint4 *>(out + r * k.ldq + c) = *reinterpret_cast<uint4 *>(h);
+  }
+}
+
+// ds = g act'(out) for eight columns; out from fp32 (`out`) or from its kept form.
+struct DsArgs {
+  const float *g, *out;
+  Kept kept;
+  int act;
+  int64_t M, N;
+  bool vec;
+};
+__device__ __forceinline__ void ds8(const DsArgs &a, int64_t r, int64_t c, float (&v)[8]) {
+  const int64_t left = a.N - c;
+  float o[8];
+  auto load = [&](const float *p, float (&t)[8]) {
+    if (a.vec && left >= 8) {
+      const float4 x = __ldg(reinterpret_cast<const float4 *>(p)), y = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+      t[0] = x.x; t[1] = x.y; t[2] = x.z; t[3] = x.w; t[4] = y.x; t[5] = y.y; t[6] = y.z; t[7] = y.w;
+    } else {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) t[u] = u < left ? __ldg(p + u) : 0.f;
+    }
+  };
+  load(a.g + r * a.N + c, v);
+  if (a.act) {
+    if (a.out) load(a.out + r * a.N + c, o);
+    else kept8(a.kept, r, c, 1.f, o);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = u < left ? v[u] * act_bwd(a.act, o[u]) : 0.f;
+  }
+}
+__global__ void __launch_bounds__(256) ds_amax_kernel(DsArgs a, uint32_t *__restrict__ amax) {
+  const int64_t per_row = (a.N + 7) / 8, total = a.M * per_row, step = (int64_t)gridDim.x * blockDim.x;
+  const bool narrow = total < ((int64_t)1 << 31);
+  uint32_t best = 0;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
+    const int64_t r = narrow ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row, c = (i - r * per_row) * 8;
+    float v[8];
+    ds8(a, r, c, v);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const uint32_t b = __float_as_uint(v[u]) & 0x7FFFFFFFu;
+      if (b < 0x7F800000u && b > best) best = b;
+    }
+  }
+  best = __reduce_max_sync(0xffffffffu, best);
+  if ((threadIdx.x & 31) == 0 && best) atomicMax(amax, best);
+}
+// The fp16 pair of ds (or ds itself, ds32) and its sums over 64 rows: a CTA takes 64 rows x 128 columns.
+__global__ void __launch_bounds__(256)
+ds_split_kernel(DsArgs a, const uint32_t *__restrict__ amax, __half *__restrict__ hi, __half *__restrict__ lo, int64_t ld,
+                float *__restrict__ ds32, float *__restrict__ sums) {
+  __shared__ float sh[16][128];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int64_t c = (int64_t)blockIdx.x * 128 + tx * 8;
+  const float s = half_scale(amax);
+  for (int64_t t = blockIdx.y; t * 64 < a.M; t += gridDim.y) {
+    float cs[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) cs[u] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t r = t * 64 + ty + 16 * j;
+      if (r < a.M && c < a.N) {
+        float v[8];
+        ds8(a, r, c, v);
+        if (hi) {
+          __half h[8], l[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) half_pair(v[u] * s, h[u], l[u]);
+          *reinterpret_cast<uint4 *>(hi + r * ld + c) = *reinterpret_cast<uint4 *>(h);
+          *reinterpret_cast<uint4 *>(lo + r * ld + c) = *reinterpret_cast<uint4 *>(l);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          if (ds32 && c + u < a.N) ds32[r * a.N + c + u] = v[u];
+          cs[u] += v[u];
+        }
+      }
+    }
+    if (sums) {
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < 8; ++u) sh[ty][tx * 8 + u] = cs[u];
+      __syncthreads();
+      if (threadIdx.x < 128) {
+        float v = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v += sh[i][threadIdx.x];
+        const int64_t n = (int64_t)blockIdx.x * 128 + threadIdx.x;
+        if (n < a.N) sums[t * a.N + n] = v;
+      }
+    }
+  }
+}
+
+// The tensor-core products take over where a product has enough work to fill a few CTA pairs.
+static bool keep_small(int64_t M, int64_t N, int64_t K) {
+  if (!gemm_f16_available()) return true;
+  return M * K <= ((int64_t)1 << 24) / N;
+}
+
+struct KeepForward { uint32_t *amax; __half *xh, *xl, *wh, *wl; float *partial; int64_t ldx, ldw; };
+static size_t keep_carve_forward(int64_t M, int64_t N, int64_t K, char *base, KeepForward &f) {
+  Carver c{base};
+  f = KeepForward{};
+  f.amax = c.take<uint32_t>(2);
+  if (!keep_small(M, N, K)) {
+    f.ldx = ceil_div(K, 8) * 8; f.ldw = ceil_div(N, 8) * 8;
+    f.xh = c.take<__half>(M * f.ldx); f.xl = c.take<__half>(M * f.ldx);
+    f.wh = c.take<__half>(K * f.ldw); f.wl = c.take<__half>(K * f.ldw);
+    f.partial = reinterpret_cast<float *>(c.take<char>((int64_t)gemm_f16_partial_bytes(M, N, K)));
+  }
+  return c.used;
+}
+struct KeepBackward { uint32_t *amax; __half *dh, *dl, *wh, *wl, *x8; float *partial, *sums, *ds32, *x32; int64_t ldd, ldw, ldx; };
+static size_t keep_carve_backward(int64_t M, int64_t N, int64_t K, char *base, KeepBackward &f) {
+  Carver c{base};
+  f = KeepBackward{};
+  f.amax = c.take<uint32_t>(2);
+  f.sums = c.take<float>(ceil_div(M, 64) * N);
+  if (keep_small(M, N, K)) {
+    f.ds32 = c.take<float>(M * N);
+    f.x32 = c.take<float>(M * K);
+  } else {
+    f.ldd = f.ldw = ceil_div(N, 8) * 8;
+    f.ldx = ceil_div(K, 32) * 32;
+    f.dh = c.take<__half>(M * f.ldd); f.dl = c.take<__half>(M * f.ldd);
+    f.wh = c.take<__half>(K * f.ldw); f.wl = c.take<__half>(K * f.ldw);
+    f.x8 = c.take<__half>(M * f.ldx);
+    const size_t a = gemm_f16_partial_bytes(M, K, N), b = gemm_f16_partial_bytes(K, N, M);
+    f.partial = reinterpret_cast<float *>(c.take<char>((int64_t)(a > b ? a : b)));
+  }
+  return c.used;
+}
+
+static int keep_check(const char *what, int64_t M, int64_t N, int64_t K, int act, const void *scratch) {
+  EB_REQUIRE(M >= 0 && N >= 0 && K >= 0, ENDIA_B200_EINVAL, "%s: negative size", what);
+  EB_REQUIRE(M <= (1 << 27) && N <= (1 << 27) && K <= (1 << 27), ENDIA_B200_ELIMIT, "%s: sizes must stay below 2^27", what);
+  EB_REQUIRE(act >= 0 && act <= ENDIA_B200_ACT_SIGMOID, ENDIA_B200_EINVAL, "%s: unknown activation %d", what, act);
+  EB_REQUIRE(scratch && (reinterpret_cast<uintptr_t>(scratch) & 255) == 0, ENDIA_B200_EINVAL,
+             "%s: scratch must be given, 256-byte aligned", what);
+  return ENDIA_B200_OK;
+}
+
+static int run_keep8(const float *x, int64_t ld, int64_t rows, int64_t cols, int keep_sign, void *kept, cudaStream_t s) {
+  EB_CUDA(cudaMemsetAsync(kept, 0, 256, s));
+  if (rows == 0 || cols == 0) return ENDIA_B200_OK;
+  const Kept k = kept_view(kept, rows, cols);
+  const int grid = grid_for(rows * (k.ldq / 4), 256, 8);
+  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ld % 4 == 0 || rows == 1);
+  if (vec) keep8_kernel<true><<<grid, 256, 0, s>>>(x, ld, rows, cols, keep_sign, k);
+  else keep8_kernel<false><<<grid, 256, 0, s>>>(x, ld, rows, cols, keep_sign, k);
+  EB_LAUNCH_CHECK();
+  return ENDIA_B200_OK;
+}
+
+}  // namespace eb
+
+extern "C" {
+
+size_t endia_b200_keep8_bytes(int64_t rows, int64_t cols) {
+  if (rows < 0 || cols < 0) return 0;
+  const size_t ldq = ((size_t)cols + 31) / 32 * 32;
+  return 256 + ((size_t)rows * (ldq + ldq / 32) + 255) / 256 * 256;
+}
+
+int endia_b200_keep8(const float *x, int64_t ldx, int64_t rows, int64_t cols, int32_t keep_sign, void *kept, void *stream) {
+  int st = require_device();
+  if (st) return st;
+  EB_REQUIRE(rows >= 0 && cols >= 0, ENDIA_B200_EINVAL, "keep8: negative size");
+  EB_REQUIRE(kept && (reinterpret_cast<uintptr_t>(kept) & 255) == 0, ENDIA_B200_EINVAL, "keep8: kept must be given, 256-byte aligned");
+  EB_REQUIRE(rows == 0 || cols == 0 || (x && ldx >= cols), ENDIA_B200_EINVAL, "keep8: NULL input or leading dimension too small");
+  return run_keep8(x, ldx, rows, cols, keep_sign, kept, as_stream(stream));
+}
+
+int endia_b200_keep8_read(const void *kept, int64_t rows, int64_t cols, float *out, void *stream) {
+  int st = require_device();
+  if (st) return st;
+  EB_REQUIRE(rows >= 0 && cols >= 0, ENDIA_B200_EINVAL, "keep8_read: negative size");
+  if (rows == 0 || cols == 0) return ENDIA_B200_OK;
+  EB_REQUIRE(kept && out, ENDIA_B200_EINVAL, "keep8_read: NULL pointer");
+  const Kept k = kept_view(const_cast<void *>(kept), rows, cols);
+  kept_read_kernel<<<grid_for(rows * (k.ldq / 8), 256, 8), 256, 0, as_stream(stream)>>>(k, rows, cols, out);
+  EB_LAUNCH_CHECK();
+  return ENDIA_B200_OK;
+}
+
+size_t endia_b200_linear_keep_scratch_bytes(int64_t M, int64_t N, int64_t K, int32_t backward) {
+  if (M < 0 || N < 0 || K < 0 || M > (1 << 27) || N > (1 << 27) || K > (1 << 27)) return 256;
+  if (M == 0 || N == 0 || K == 0) return 256;
+  KeepForward f;
+  KeepBackward b;
+  return backward ? keep_carve_backward(M, N, K, nullptr, b) : keep_carve_forward(M, N, K, nullptr, f);
+}
+
+int endia_b200_linear_keep_fwd(const float *x, int64_t ldx, const float *W, int64_t ldw, const float *bias, int32_t act,
+                               int64_t M, int64_t N, int64_t K, float *out, void *kept_x, int32_t keep_sign,
+                               void *scratch, void *stream) {
+  int st = require_device();
+  if (st) return st;
+  if ((st = keep_check("linear_keep", M, N, K, act, scratch))) return st;
+  EB_REQUIRE(K >= 1, ENDIA_B200_EINVAL, "linear_keep: needs at least one input feature");
+  EB_REQUIRE(!kept_x || (reinterpret_cast<uintptr_t>(kept_x) & 255) == 0, ENDIA_B200_EINVAL, "linear_keep: kept_x must be 256-byte aligned");
+  cudaStream_t s = as_stream(stream);
+  if (M == 0) return kept_x ? run_keep8(x, ldx, M, K, keep_sign, kept_x, s) : ENDIA_B200_OK;
+  EB_REQUIRE(x && ldx >= K && (N == 0 || (W && out && ldw >= N)), ENDIA_B200_EINVAL, "linear_keep: NULL pointer or leading dimension too small");
+  if (kept_x && (st = run_keep8(x, ldx, M, K, keep_sign, kept_x, s))) return st;
+  if (N == 0) return ENDIA_B200_OK;
+  if (keep_small(M, N, K)) return gemm_fp32(0, 0, M, N, K, x, ldx, W, ldw, out, N, bias, act, 0.f, s);
+  KeepForward f;
+  keep_carve_forward(M, N, K, static_cast<char *>(scratch), f);
+  EB_CUDA(cudaMemsetAsync(f.amax, 0, 2 * sizeof(uint32_t), s));
+  if ((st = launch_amax(x, M, K, ldx, nullptr, f.amax, s))) return st;
+  if ((st = launch_amax(W, K, N, ldw, nullptr, f.amax + 1, s))) return st;
+  if ((st = launch_half_split(x, M, K, ldx, nullptr, f.amax, f.xh, f.xl, f.ldx, s))) return st;
+  if ((st = launch_half_split(W, K, N, ldw, nullptr, f.amax + 1, f.wh, f.wl, f.ldw, s))) return st;
+  F16Gemm g;
+  g.M = M; g.N = N; g.K = K;
+  g.a = HalfPair{f.xh, f.xl, f.ldx, f.amax};
+  g.b = HalfPair{f.wh, f.wl, f.ldw, f.amax + 1};
+  g.bias = bias; g.act = act; g.C = out; g.ldc = N; g.partial = f.partial;
+  return launch_gemm_f16(g, false, true, F16_STORE, s);
+}
+
+int endia_b200_linear_keep_bwd(const void *kept_x, const float *W, int64_t ldw, const float *out, const void *kept_out,
+                               int32_t act, const float *grad, int64_t M, int64_t N, int64_t K, float *dx, float *dw,
+                               float *db, void *scratch, void *stream) {
+  int st = require_device();
+  if (st) return st;
+  if ((st = keep_check("linear_keep", M, N, K, act, scratch))) return st;
+  EB_REQUIRE(K >= 1, ENDIA_B200_EINVAL, "linear_keep: needs at least one input feature");
+  cudaStream_t s = as_stream(stream);
+  if (M == 0 || N == 0) {
+    if (dx && M) EB_CUDA(cudaMemsetAsync(dx, 0, sizeof(float) * (size_t)M * (size_t)K, s));
+    if (dw && N) EB_CUDA(cudaMemsetAsync(dw, 0, sizeof(float) * (size_t)K * (size_t)N, s));
+    if (db && N) EB_CUDA(cudaMemsetAsync(db, 0, sizeof(float) * (size_t)N, s));
+    return ENDIA_B200_OK;
+  }
+  if (!dx && !dw && !db) return ENDIA_B200_OK;
+  EB_REQUIRE(grad && (!dw || kept_x) && (!dx || (W && ldw >= N)) && (act == 0 || out || kept_out), ENDIA_B200_EINVAL,
+             "linear_keep: NULL pointer or leading dimension too small");
+  KeepBackward f;
+  keep_carve_backward(M, N, K, static_cast<char *>(scratch), f);
+  const bool small = keep_small(M, N, K);
+  DsArgs a{};
+  a.g = grad; a.out = act && out ? out : nullptr; a.act = act; a.M = M; a.N = N;
+  if (act && !out) a.kept = kept_view(const_cast<void *>(kept_out), M, N);
+  a.vec = N % 4 == 0 && (reinterpret_cast<uintptr_t>(grad) & 15) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  const dim3 grid((unsigned)ceil_div(N, 128), (unsigned)(ceil_div(M, 64) < 32768 ? ceil_div(M, 64) : 32768));
+  if (!small) {
+    EB_CUDA(cudaMemsetAsync(f.amax, 0, 2 * sizeof(uint32_t), s));
+    ds_amax_kernel<<<grid_for(M * ceil_div(N, 8), 256, 8), 256, 0, s>>>(a, f.amax);
+    EB_LAUNCH_CHECK();
+  }
+  ds_split_kernel<<<grid, 256, 0, s>>>(a, f.amax, f.dh, f.dl, f.ldd, f.ds32, db ? f.sums : nullptr);
+  EB_LAUNCH_CHECK();
+  if (db && (st = launch_colsum_finish(f.sums, db, N, (int)ceil_div(M, 64), 1, s))) return st;
+  const Kept kx = kept_view(const_cast<void *>(kept_x), M, K);
+  if (small) {
+    if (dx && (st = gemm_fp32(0, 1, M, K, N, f.ds32, N, W, ldw, dx, K, nullptr, 0, 0.f, s))) return st;
+    if (dw) {
+      kept_read_kernel<<<grid_for(M * (kx.ldq / 8), 256, 8), 256, 0, s>>>(kx, M, K, f.x32);
+      EB_LAUNCH_CHECK();
+      return gemm_fp32(1, 0, K, N, M, f.x32, K, f.ds32, N, dw, N, nullptr, 0, 0.f, s);
+    }
+    return ENDIA_B200_OK;
+  }
+  const HalfPair d{f.dh, f.dl, f.ldd, f.amax};
+  if (dw) {
+    kept_half_kernel<<<grid_for(M * (kx.ldq / 8), 256, 8), 256, 0, s>>>(kx, M, f.x8);
+    EB_LAUNCH_CHECK();
+    F16Gemm g;
+    g.M = K; g.N = N; g.K = M;
+    g.a = HalfPair{f.x8, nullptr, f.ldx, kx.amax};
+    g.b = d;
+    g.C = dw; g.ldc = N; g.partial = f.partial;
+    if ((st = launch_gemm_f16(g, true, true, F16_STORE, s))) return st;
+  }
+  if (dx) {
+    if ((st = launch_amax(W, K, N, ldw, nullptr, f.amax + 1, s))) return st;
+    if ((st = launch_half_split(W, K, N, ldw, nullptr, f.amax + 1, f.wh, f.wl, f.ldw, s))) return st;
+    F16Gemm g;
+    g.M = M; g.N = K; g.K = N;
+    g.a = d;
+    g.b = HalfPair{f.wh, f.wl, f.ldw, f.amax + 1};
+    g.C = dx; g.ldc = K; g.partial = f.partial;
+    if ((st = launch_gemm_f16(g, false, false, F16_STORE, s))) return st;
+  }
+  return ENDIA_B200_OK;
+}
+
+}  // extern "C"

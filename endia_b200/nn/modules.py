@@ -9,6 +9,7 @@ from ..functional import init_ops
 from ..functional._utils import op_array, setup_shape_and_data, contiguous
 from ..functional.binary_ops import matmul, mul, add, gemm_arrays
 from ..functional.comparison_ops import greater
+from ..functional.keep_ops import keep8
 from ..functional.reduce_ops import reduce_add
 from ..functional.unary_ops import relu, tanh, sigmoid, square
 
@@ -54,10 +55,15 @@ def _act_bwd_graph(act, out, grad):
     return grad
 
 
-def linear(x, weight, bias=None, activation=None):
+def linear(x, weight, bias=None, activation=None, checkpoint=False):
     """act(x @ weight + bias) for 2-D x (B, K), weight (K, N), bias (N). Other ranks use the
-    unfused op composition of the reference (_mlp.mojo:50-52)."""
+    unfused op composition of the reference (_mlp.mojo:50-52).
+
+    checkpoint=True: the layer keeps its input for the backward pass in 8 bits and reads no float32
+    activation there (see _linear_kept and keep8)."""
     act = _ACTS[activation]
+    if checkpoint:
+        return _linear_kept(x, weight, bias, act)
     if x.ndim() != 2 or weight.ndim() != 2 or (bias is not None and bias.ndim() != 1) or x.is_complex() \
             or weight.is_complex():
         pred = matmul(x, weight)
@@ -185,6 +191,80 @@ def linear(x, weight, bias=None, activation=None):
     return res
 
 
+def _linear_kept(x, weight, bias, act):
+    """The layer of linear(..., checkpoint=True): out = act(x @ weight + bias) from x itself, in products
+    of 22-bit operand pairs (errors of some 2^-22, less than linear's); the backward pass uses the
+    8-bit form of x (dW = x8^T ds) and, when `out` has been handed to keep8, of out (the
+    activation's derivative; exact for ReLU). x itself stays as it is: keep8(x) releases its float32
+    storage once nothing else needs it. With create_graph=True the VJP is the composition of
+    differentiable ops, on whatever x and out then hold."""
+    from ..functional.keep_ops import Kept8, quantise, keeps_sign
+    from ..functional.loss_ops import _row_major, _scratch
+    if x.ndim() != 2 or weight.ndim() != 2 or (bias is not None and bias.ndim() != 1) or \
+            any(a.is_complex() for a in [x, weight] + ([bias] if bias is not None else [])):
+        raise _lib.EndiaError(_lib.EINVAL, "linear: checkpoint=True takes real arrays x (B, K), weight (K, N), bias (N)")
+    if x.shape()[1] != weight.shape()[0] or (bias is not None and bias.shape()[0] != weight.shape()[1]):
+        raise _lib.EndiaError(_lib.ESHAPE, "linear: incompatible shapes %s @ %s + %s" % (
+            x.shape(), weight.shape(), bias.shape() if bias is not None else None))
+    (B, K), N = x.shape(), weight.shape()[1]
+    if K == 0:
+        raise _lib.EndiaError(_lib.ESHAPE, "linear: checkpoint=True needs at least one input feature")
+    args = [x, weight] + ([bias] if bias is not None else [])
+    saved = {}
+
+    def call(curr, a):
+        setup_shape_and_data(curr)
+        xr, ldx = _row_major(a[0])
+        wr, ldw = _row_major(a[1])
+        b = contiguous(a[2]) if bias is not None else None
+        kept = None
+        if curr.requires_grad_flag:
+            kept = saved["x"] = alloc((_lib.lib.endia_b200_keep8_bytes(B, K) + 3) // 4)
+            a[0]._kept8 = kept
+        scratch = _scratch(_lib.lib.endia_b200_linear_keep_scratch_bytes(B, N, K, 0))
+        _lib.call("endia_b200_linear_keep_fwd", xr.data_ptr(), ldx, wr.data_ptr(), ldw,
+                  b.data_ptr() if b is not None else None, act, B, N, K, curr.data_ptr(),
+                  kept.data_ptr() if kept is not None else None, int(keeps_sign(a[0])), scratch.data_ptr(), stream())
+
+    def vjp(primals, grad, out):
+        xp, wp = primals[0], primals[1]
+        zero = Array(0)
+        want = [_state.wants_grad(p) for p in primals]
+        if _state.create_graph:
+            ds = _act_bwd_graph(act, out, grad)
+            res = [matmul(ds, wp.T()) if want[0] else zero, matmul(xp.T(), ds) if want[1] else zero]
+            if bias is not None:
+                res.append(reduce_add(ds, [0]) if want[2] else zero)
+            return res
+        res = []
+        for w, shape in zip(want, ([B, K], [K, N], [1, N])):      # (bias gradient: kept dim, like Expand.vjp)
+            res.append(zero)
+            if w:
+                res[-1] = Array(ArrayShape(shape))
+                setup_shape_and_data(res[-1])
+        if any(want):
+            g = contiguous(grad)
+            wr, ldw = _row_major(wp)
+            held = isinstance(out, Kept8) and out.held()
+            o = None if held or not act else contiguous(out)
+            scratch = _scratch(_lib.lib.endia_b200_linear_keep_scratch_bytes(B, N, K, 1))
+            ptrs = [r.data_ptr() if w else None for r, w in zip(res, want)] + [None]
+            _lib.call("endia_b200_linear_keep_bwd", saved["x"].data_ptr(), wr.data_ptr(), ldw,
+                      o.data_ptr() if o is not None else None, out._kept8.data_ptr() if held else None, act, g.data_ptr(),
+                      B, N, K, *ptrs[:3], scratch.data_ptr(), stream())
+        return res
+
+    def jvp(primals, tangents):
+        z = matmul(primals[0], primals[1])
+        dz = add(matmul(tangents[0], primals[1]), matmul(primals[0], tangents[1]))
+        if bias is not None:
+            z, dz = add(z, primals[2]), add(dz, tangents[2])
+        return _act_bwd_graph(act, _ACT_FNS[act](z), dz) if act else dz
+    res = op_array(ArrayShape([B, N]), args, "linear_kept", call, vjp=vjp, jvp=jvp)
+    res._lin_act = act
+    return res
+
+
 def _mask_epilogue_for(xp, dx):
     """When the input `xp` of a linear layer is itself the output of a fused linear layer with
     this layer as its only consumer, the dX product can finish that layer's backward step in its
@@ -224,14 +304,18 @@ def _mask_epilogue_for(xp, dx):
 
 class MLP:
     """Stack of linear layers (weights stored (in, out)); `activation` on all but the last layer.
-    The reference hard-codes ReLU and He-normal initialisation (_mlp.mojo:34-43, 52)."""
+    The reference hard-codes ReLU and He-normal initialisation (_mlp.mojo:34-43, 52).
 
-    def __init__(self, hidden_dims, compute_backward=False, activation="relu"):
+    checkpoint=True: the activations between the layers are held in 8 bits for the backward pass (8.25
+    bits per value instead of 32); the forward values are not touched by it."""
+
+    def __init__(self, hidden_dims, compute_backward=False, activation="relu", checkpoint=False):
         self.weights, self.biases = [], []
         self.hidden_dims = list(hidden_dims)
         self.num_layers = len(hidden_dims) - 1
         self.compute_backward = compute_backward
         self.activation = activation
+        self.checkpoint = checkpoint
         for i in range(self.num_layers):
             self.weights.append(init_ops.rand_he_normal([hidden_dims[i], hidden_dims[i + 1]],
                                                         fan_in=hidden_dims[i],
@@ -240,11 +324,7 @@ class MLP:
                                                        requires_grad=compute_backward))
 
     def forward(self, x):
-        pred = x
-        for i in range(self.num_layers):
-            last = i == self.num_layers - 1
-            pred = linear(pred, self.weights[i], self.biases[i], None if last else self.activation)
-        return pred
+        return _layers(x, list(zip(self.weights, self.biases)), self.activation, self.checkpoint)
 
     __call__ = forward
 
@@ -259,13 +339,21 @@ class MLP:
                        for i, (w, b) in enumerate(zip(self.weights, self.biases)))
 
 
-def mlp(args, activation="relu"):
-    """Functional form: args = [x, target, W0, b0, W1, b1, ...] (_mlp.mojo:71-82)."""
-    pred = args[0]
+def mlp(args, activation="relu", checkpoint=False):
+    """Functional form: args = [x, target, W0, b0, W1, b1, ...] (_mlp.mojo:71-82); checkpoint as in MLP."""
     num_layers = (len(args) - 2) // 2
-    for i in range(num_layers):
-        last = i == num_layers - 1
-        pred = linear(pred, args[2 * i + 2], args[2 * i + 3], None if last else activation)
+    return _layers(args[0], [(args[2 * i + 2], args[2 * i + 3]) for i in range(num_layers)], activation, checkpoint)
+
+
+def _layers(x, params, activation, checkpoint):
+    """`activation` on all but the last layer. With `checkpoint` an activation is handed to keep8 as soon
+    as the layer above has used it (x itself is the caller's)."""
+    pred = x
+    for i, (w, b) in enumerate(params):
+        below = pred
+        pred = linear(below, w, b, None if i == len(params) - 1 else activation, checkpoint)
+        if checkpoint and i > 0 and below.requires_grad():
+            keep8(below)
     return pred
 
 

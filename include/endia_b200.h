@@ -311,6 +311,68 @@ int endia_b200_act_bwd_colsum_parts(int act, const float *act_out, const float *
                                     float *colsum, int64_t M, int64_t N, void *scratch, void *pair16,
                                     void *stream);
 
+/* -------------------------------------- cross entropy over a large vocabulary ---- */
+
+enum { ENDIA_B200_LOSS_MEAN = 0, ENDIA_B200_LOSS_SUM = 1, ENDIA_B200_LOSS_NONE = 2 };
+
+/* Softmax cross entropy of the rows of x W + b against class numbers, without an array of the logits:
+ *   l = x W + b,  loss_m = log sum_v exp(l[m,v]) - l[m, t(m)]
+ * x is [M, K] (leading dimension ldx >= K), W [K, V] (ldw >= V), bias [V] or NULL, target [M]: class
+ * numbers as floats. target[m] < 0: the row is left out (its loss and its row of dx are 0, it adds
+ * nothing to dw and db, whatever its x holds). A target that is not an integer below V (NaN included)
+ * makes the row's loss and all gradients it takes part in NaN. Logits of -inf (a bias that bans a class)
+ * have probability 0.
+ *   reduction MEAN: loss[0] = sum / number of rows that count (0 when none does);  SUM: loss[0] = sum;
+ *   NONE: loss[M], one per row
+ * `state` (endia_b200_linear_ce_state_bytes(M) bytes) carries what the backward call needs besides the
+ * inputs (log-sum-exp per row, the count, the operands' scales); x, W, bias and target must be
+ * unchanged then. `grad` is the incoming gradient: one float (MEAN, SUM) or M floats (NONE).
+ *   dx [M, K], dw [K, V], db [V], all contiguous, each may be NULL (not computed)
+ * `scratch`: endia_b200_linear_ce_scratch_bytes(M, K, V, backward) bytes, 256-byte aligned: the
+ * vocabulary is walked in equal pieces whose work space stays near 256 MiB (pieces of at least 1024
+ * columns). Limits: V <= 2^24 (class numbers are float32 values), M and K below 2^27. The order of
+ * every sum is fixed: the same inputs give the same bits.
+ * Accuracy: products of 22-bit operand pairs summed in fp32 (fp32 kernels for small problems).
+ * No counterpart in the reference, whose one loss is mse (endia/functional/loss_ops/mse_op.mojo:18-20). */
+size_t endia_b200_linear_ce_state_bytes(int64_t M);
+size_t endia_b200_linear_ce_scratch_bytes(int64_t M, int64_t K, int64_t V, int32_t backward);
+int endia_b200_linear_ce_fwd(const float *x, int64_t ldx, const float *W, int64_t ldw, const float *bias,
+                             const float *target, int64_t M, int64_t K, int64_t V, int32_t reduction, float *loss,
+                             float *state, void *scratch, void *stream);
+int endia_b200_linear_ce_bwd(const float *x, int64_t ldx, const float *W, int64_t ldw, const float *bias,
+                             const float *target, int64_t M, int64_t K, int64_t V, int32_t reduction, const float *grad,
+                             const float *state, float *dx, float *dw, float *db, void *scratch, void *stream);
+
+/* ------------------------------------------------ activations held in 8 bits ---- */
+
+/* The 8-bit form of an array of `rows` x `cols` floats (leading dimension ldx) for a backward pass:
+ * blocks of 32 consecutive columns share a power of two,
+ *   x ~ q * 2^e,  e = the smallest integer >= -126 with round(max|x| / 2^e) <= 127,  q = round(x / 2^e)
+ * (half to even). keep_sign != 0: a value that is not zero keeps |q| >= 1, so that the derivative of a
+ * ReLU taken from its kept output is exact. Infinite and NaN values read back as NaN (and do not count
+ * in max|x|). `kept` holds endia_b200_keep8_bytes(rows, cols) bytes (8.25 bits per value), 256-byte
+ * aligned. keep8_read writes the values it stands for, contiguous [rows, cols]. */
+size_t endia_b200_keep8_bytes(int64_t rows, int64_t cols);
+int endia_b200_keep8(const float *x, int64_t ldx, int64_t rows, int64_t cols, int32_t keep_sign, void *kept, void *stream);
+int endia_b200_keep8_read(const void *kept, int64_t rows, int64_t cols, float *out, void *stream);
+
+/* A linear layer whose backward pass reads 8-bit forms instead of float32 activations:
+ *   fwd: out[M,N] = act(x[M,K] W[K,N] + bias[N]); kept_x (optional) receives the 8-bit form of x
+ *   bwd: ds = grad * act'(out);  dx = ds W^T,  dw = x8^T ds,  db[N] = sum over the rows of ds
+ * with act' as in endia_b200_epilogue, taken from `out` (fp32) or, when that is NULL, from `kept_out`.
+ * out, grad, dx, dw, db are contiguous; dx, dw and db may be NULL. `scratch`:
+ * endia_b200_linear_keep_scratch_bytes(M, N, K, backward) bytes, 256-byte aligned. Sizes below 2^27,
+ * K >= 1. The order of every sum is fixed. Replaces, for such a layer, the forward loop of matmul_fwd
+ * (matmul_op.mojo:93-254), the products of matmul_vjp (:278-284) and the masks of the activations'
+ * VJPs (relu_op.mojo:95, tanh_op.mojo:92, sigmoid_op.mojo:98); the 8-bit form has no counterpart. */
+size_t endia_b200_linear_keep_scratch_bytes(int64_t M, int64_t N, int64_t K, int32_t backward);
+int endia_b200_linear_keep_fwd(const float *x, int64_t ldx, const float *W, int64_t ldw, const float *bias, int32_t act,
+                               int64_t M, int64_t N, int64_t K, float *out, void *kept_x, int32_t keep_sign,
+                               void *scratch, void *stream);
+int endia_b200_linear_keep_bwd(const void *kept_x, const float *W, int64_t ldw, const float *out, const void *kept_out,
+                               int32_t act, const float *grad, int64_t M, int64_t N, int64_t K, float *dx, float *dw,
+                               float *db, void *scratch, void *stream);
+
 /* --------------------------------------------------------------- optimizer ---- */
 
 /* One fused Adam step over n_tensors parameter tensors (device pointers passed in HOST arrays):
