@@ -11,8 +11,10 @@
 // Per stage the tensor pipe is busy for 12 x 128 = 1536 cycles; the drain of 256 columns by eight warps
 // takes about a third of that, so it costs no tensor time. What it buys: errors of 2e-7 instead of
 // 1e-5 at K = 4096, at 3 fp16 MMAs per product (tf32 + 2 bf16 take the time of 4).
-//   warp 0: TMA producer (one lane), warp 1: MMA issuer (one lane of the leader CTA),
-//   warps 2-9: sums, epilogue and stores (lane quarter warp & 3, column half (warp - 2) >> 2).
+//   warp 0: TMA producer (one lane), warp 1: MMA issuer (one lane of the leader CTA), warps 2, 3 idle
+//   warps 4-11: sums, epilogue and stores (lane quarter warp & 3, column half (warp - 4) >> 2)
+// The 168 registers a thread that the launch hands out are split as 56 for the first warpgroup and 224
+// for the other two (128 sums, 64 in flight from tensor memory).
 // Every wait is bounded; a wait that gives up records a code, the CTA drains its copies and returns.
 #include "gemm_f16.cuh"
 #include "gemm.cuh"
@@ -23,6 +25,9 @@ namespace eb {
 constexpr int F16_BK = 64;                       // one stage: 64 of K, 128 bytes per K-major row
 constexpr uint32_t F16_TILE = 128 * F16_BK * 2;  // bytes of one [128 x 64] fp16 tile
 constexpr int F16_EPI_WARPS = 8;
+constexpr int F16_THREADS = 384;
+constexpr int F16_REGS_CONTROL = 56, F16_REGS_EPI = 224;
+static_assert(F16_REGS_CONTROL * 128 + F16_REGS_EPI * 256 <= 168 * F16_THREADS, "registers of the launch");
 
 struct F16Maps {
   CUtensorMap a_hi, a_lo, b_hi, b_lo;
@@ -81,7 +86,7 @@ __device__ __forceinline__ float warp_colsum32(float (&v)[32], int lane) {
 
 // PROD: 3 = both operands are pairs, 2 = A is exact in its hi part.
 template <bool A_MN, bool B_MN, int PROD, int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F16_THREADS, 1)
 gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
   constexpr int STAGES = PROD == 3 ? 3 : 4;
   constexpr uint32_t A_BYTES = (PROD == 3 ? 2 : 1) * F16_TILE, STAGE_BYTES = A_BYTES + 2 * F16_TILE;
@@ -132,6 +137,8 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
   tc_fence_after();
   const uint32_t tmem_base = tmem_slot;
 
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F16_REGS_CONTROL));
   if (warp == 0) {
     if (lane == 0) {
       uint32_t it = 0;
@@ -174,7 +181,7 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
         k_range(t, kb, kb1);
         for (; kb < kb1; ++kb, ++j) {
           const int s = (int)(j % STAGES), b = (int)(j & 1);
-          if (j >= 2 && !mbar_wait_cluster(acc_empty(b), ((j >> 1) - 1) & 1, 53)) { ok = false; break; }
+          if (j >= 2 && !mbar_wait(acc_empty(b), ((j >> 1) - 1) & 1, 53)) { ok = false; break; }
           if (!mbar_wait(full_bar(s), (j / STAGES) & 1, 54)) { ok = false; break; }
           tc_fence_after();
           const uint32_t st = smem_base + s * STAGE_BYTES, sb = st + A_BYTES, d = tmem_base + 256u * b;
@@ -196,9 +203,11 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
         }
       }
     }
+  }
   } else {
-    const int q = warp & 3, half = (warp - 2) >> 2;
-    const uint32_t ebuf = epi_base + (uint32_t)(warp - 2) * 4096u;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F16_REGS_EPI));
+    const int q = warp & 3, half = (warp - 4) >> 2;
+    const uint32_t ebuf = epi_base + (uint32_t)(warp - 4) * 4096u;
     const uint32_t row_addr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * 128);
     const uint32_t empty_leader[2] = {map_to_cta(acc_empty(0), 0), map_to_cta(acc_empty(1), 0)};
     const float f0 = half_unscale(p.amax_a);
@@ -217,16 +226,22 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
         if (!mbar_wait(acc_full((int)b), (j >> 1) & 1, 55)) { ok = false; break; }
         tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t r[32];
-          tc_ld32(row_addr + 256u * b + (uint32_t)(32 * c), r);
+        for (int c = 0; c < 4; c += 2) {
+          uint32_t r0[32], r1[32];
+          tc_ld32(row_addr + 256u * b + (uint32_t)(32 * c), r0);
+          tc_ld32(row_addr + 256u * b + (uint32_t)(32 * c + 32), r1);
           tc_wait_ld();
+          if (c == 2) {       // the last values have left tensor memory
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote(empty_leader[b]);
+          }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) acc[32 * c + i] += __uint_as_float(r[i]);
+          for (int i = 0; i < 32; ++i) {
+            acc[32 * c + i] += __uint_as_float(r0[i]);
+            acc[32 * c + 32 + i] += __uint_as_float(r1[i]);
+          }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(empty_leader[b]);
       }
       if (!ok) break;
       const int nb = n0 + half * 128;            // this warp's first column
@@ -548,7 +563,7 @@ static int launch_kernel(const F16Maps &maps, const F16Params &p, cudaStream_t s
     EB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2);
-    cfg.blockDim = dim3(320);
+    cfg.blockDim = dim3(F16_THREADS);
     cfg.dynamicSmemBytes = SMEM;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeClusterDimension;
@@ -563,7 +578,7 @@ static int launch_kernel(const F16Maps &maps, const F16Params &p, cudaStream_t s
     max_pairs = nc;
   }
   const int items = p.pairs_m * p.tiles_n * p.ksplit, pairs = items < max_pairs ? items : max_pairs;
-  kern<<<dim3((unsigned)(2 * pairs)), 320, SMEM, s>>>(maps, p);
+  kern<<<dim3((unsigned)(2 * pairs)), F16_THREADS, SMEM, s>>>(maps, p);
   EB_LAUNCH_CHECK();
   return ENDIA_B200_OK;
 }

@@ -159,6 +159,11 @@ __device__ __forceinline__ void tc_mma_16bit_pair(uint32_t d_tmem, uint64_t a_de
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
+// An arrival at another CTA's barrier that orders nothing but tensor-memory accesses (with the tcgen05
+// fences around it): the cluster-scope release above costs a memory barrier per arrival.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
 // Bounded wait that acquires at cluster scope (the arrivals come from both CTAs of the pair).
 __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, int code) {
   for (uint32_t it = 0; it < TC_WAIT_LIMIT; ++it) {
