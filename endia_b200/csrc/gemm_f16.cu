@@ -32,7 +32,7 @@ static_assert(F16_REGS_CONTROL * 128 + F16_REGS_EPI * 256 <= 168 * F16_THREADS, 
 struct F16Maps {
   CUtensorMap a_hi, a_lo, b_hi, b_lo;
   CUtensorMap c;           // F16_STORE: C or the work space, boxes of [32 rows][32 floats]
-  CUtensorMap d_hi, d_lo;  // F16_DLOGITS: boxes of [32 rows][64 halfs]
+  CUtensorMap d_hi, d_lo;  // F16_DLOGITS: boxes of [32 rows][32 halfs]
 };
 
 struct F16Params {
@@ -82,6 +82,17 @@ __device__ __forceinline__ float warp_colsum32(float (&v)[32], int lane) {
     }
   }
   return v[0];
+}
+
+constexpr float LOG2E = 1.4426950408889634f;
+// 2^x in one instruction (results below 2^-126 are zero)
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void sts128u(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
 // PROD: 3 = both operands are pairs, 2 = A is exact in its hi part.
@@ -212,6 +223,10 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
     const uint32_t empty_leader[2] = {map_to_cta(acc_empty(0), 0), map_to_cta(acc_empty(1), 0)};
     const float f0 = half_unscale(p.amax_a);
     const float f1 = half_unscale(p.amax_b) * (p.alpha_dev ? __ldg(p.alpha_dev) : 1.f);
+    // For logits one factor: where 2^-(e_a + e_b) leaves the range of fp32 it is held at the range's end (the
+    // logits are then below 2^-80, or beyond what their fp32 sum could hold)
+    const int e_ce = -((p.amax_a ? half_scale_exponent(*p.amax_a) : 0) + (p.amax_b ? half_scale_exponent(*p.amax_b) : 0));
+    const float f_ce = pow2f_exact(e_ce < -126 ? -126 : (e_ce > 126 ? 126 : e_ce)) * LOG2E;
     uint32_t j = 0;
     bool ok = true;
     for (int t = pair_id; t < num_items && ok; t += num_pairs) {
@@ -304,88 +319,100 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
         const bool row_ok = m < p.M;
         const float tg = row_ok ? __ldg(p.target + m) : -1.f;
         const int64_t v0 = p.n_base + nb;
-        // this lane's target among the warp's 128 columns, or a number that no column has
+        // this lane's target among the warp's 128 columns, or -1
         const int tl = (tg >= (float)v0 && tg < (float)(v0 + 128)) ? (int)((int64_t)tg - v0) : -1;
+        const bool any_target = __any_sync(0xffffffffu, tl >= 0);
+        // Logits are kept in units of log2 e (f_ce holds the factor), so that an exponential is one
+        // MUFU operation on a difference: a rounding of 2^-24 of the logit, as in any fp32 logit.
         float bv[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) bv[c] = (p.bias && nb + 32 * c + lane < p.N) ? __ldg(p.bias + nb + 32 * c + lane) : 0.f;
-        const bool has_bias = p.bias != nullptr;
-#pragma unroll
-        for (int i = 0; i < 128; ++i) {
-          acc[i] = (acc[i] * f0) * f1;
-          if (has_bias) acc[i] += __shfl_sync(0xffffffffu, bv[i >> 5], i & 31);
-        }
+        for (int c = 0; c < 4; ++c) bv[c] = p.bias && nb + 32 * c + lane < p.N ? __ldg(p.bias + nb + 32 * c + lane) * LOG2E : 0.f;
         if constexpr (EPI == F16_STATS) {
-          // the sum of 128 exponentials below a maximum of their own; -inf columns (banned classes) add 0
-          float mx = -INFINITY, tv = 0.f;
-          bool nan = false;
+          if (p.bias) {
 #pragma unroll
-          for (int i = 0; i < 128; ++i) {
-            if (nb + i >= p.N) acc[i] = -INFINITY;
-            nan |= acc[i] != acc[i];
-            mx = fmaxf(mx, acc[i]);
-            if (i == tl) tv = acc[i];
-          }
-          float sum = 0.f;
-          if (mx > -INFINITY) {
+            for (int i = 0; i < 128; ++i) acc[i] = fmaf(acc[i], f_ce, __shfl_sync(0xffffffffu, bv[i >> 5], i & 31));
+          } else {
 #pragma unroll
-            for (int i = 0; i < 128; ++i) sum += __expf(acc[i] - mx);
+            for (int i = 0; i < 128; ++i) acc[i] *= f_ce;
           }
-          if (nan) sum = NAN;
-          if (row_ok) {
-            p.stats[(v0 >> 7) * (int64_t)p.M + m] = make_float2(mx, sum);
+          if (nb + 128 > p.N) {
+#pragma unroll
+            for (int i = 0; i < 128; ++i)
+              if (nb + i >= p.N) acc[i] = -INFINITY;
+          }
+          if (any_target) {
+            float tv = 0.f;
+#pragma unroll
+            for (int i = 0; i < 128; ++i)
+              if (i == tl) tv = acc[i];
             if (tl >= 0) p.target_logit[m] = tv;
           }
+          // maximum and sum of exponentials, four chains each; -inf columns (banned classes) add 0, a NaN
+          // makes the sum NaN
+          float mx4[4] = {acc[0], acc[1], acc[2], acc[3]}, s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 4; i < 128; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], acc[i]);
+          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+          const float base = mx == -INFINITY ? 0.f : mx;      // (a row of -inf: 2^-inf = 0)
+#pragma unroll
+          for (int i = 0; i < 128; ++i) s4[i & 3] += exp2_fast(acc[i] - base);
+          if (row_ok) p.stats[(v0 >> 7) * (int64_t)p.M + m] = make_float2(mx, (s4[0] + s4[1]) + (s4[2] + s4[3]));
         } else {
           const float lse = row_ok ? __ldg(p.lse + m) : 0.f, cf = row_ok ? __ldg(p.coef + m) : 0.f;
-          const bool dead = cf == 0.f;     // a row that is left out: exactly zero, whatever its logits are
+          const bool any_dead = __any_sync(0xffffffffu, cf == 0.f);
+          const float cs = cf * F16_D_SCALE;
 #pragma unroll
-          for (int i = 0; i < 128; ++i) {
-            const float e = expf(acc[i] - lse) - (i == tl ? 1.f : 0.f);
-            acc[i] = dead ? 0.f : e * cf;
-          }
-          // hi and lo of two chunks of 64 columns through the warp's buffer
+          for (int c = 0; c < 4; ++c) {
+            const int nc = nb + 32 * c;
+            if (nc >= p.N || mq >= p.M) continue;      // (uniform over the warp)
+            float v[32];
+            // p = 2^(l - lse), d = (p - [target]) coef
+            if (p.bias) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            if (nb + 64 * c < p.N && mq < p.M) {
+              for (int i = 0; i < 32; ++i) v[i] = exp2_fast(fmaf(acc[32 * c + i], f_ce, __shfl_sync(0xffffffffu, bv[c], i) - lse));
+            } else {
 #pragma unroll
-              for (int part = 0; part < 2; ++part) {
-                if (lane == 0) bulk_wait_read0();
-                __syncwarp();
-#pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                  uint32_t w[4];
-#pragma unroll
-                  for (int k = 0; k < 4; ++k) {
-                    const float x0 = acc[64 * c + 8 * u + 2 * k] * F16_D_SCALE, x1 = acc[64 * c + 8 * u + 2 * k + 1] * F16_D_SCALE;
-                    __half2 h = __floats2half2_rn(x0, x1);
-                    if (part) {
-                      const float2 hf = __half22float2(h);
-                      h = __floats2half2_rn(x0 - hf.x, x1 - hf.y);
-                    }
-                    w[k] = *reinterpret_cast<uint32_t *>(&h);
-                  }
-                  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
-                               ::"r"(ebuf + (uint32_t)lane * 128u + (uint32_t)((u ^ (lane & 7)) * 16)),
-                               "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-                }
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                  tma_store_2d(part ? &maps.d_lo : &maps.d_hi, ebuf, nb + 64 * c, mq);
-                  bulk_commit();
-                }
-              }
+              for (int i = 0; i < 32; ++i) v[i] = exp2_fast(fmaf(acc[32 * c + i], f_ce, -lse));
             }
-          }
-          if (p.colsum_part && mq < p.M) {
+            if (any_target) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              float v[32];
+              for (int i = 0; i < 32; ++i)
+                if (32 * c + i == tl) v[i] -= 1.f;
+            }
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = acc[32 * c + i];
+            for (int i = 0; i < 32; ++i) v[i] *= cs;
+            if (any_dead) {      // rows that are left out: exactly zero, whatever their logits are
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = cf == 0.f ? 0.f : v[i];
+            }
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+              const __half2 h = __floats2half2_rn(v[2 * u], v[2 * u + 1]);
+              const float2 hf = __half22float2(h);
+              const __half2 l = __floats2half2_rn(v[2 * u] - hf.x, v[2 * u + 1] - hf.y);
+              hi[u] = *reinterpret_cast<const uint32_t *>(&h);
+              lo[u] = *reinterpret_cast<const uint32_t *>(&l);
+            }
+            // both parts of [32 rows][32 columns] through the warp's buffer, 64-byte rows, 64-byte swizzle
+            if (lane == 0) bulk_wait_read0();      // the previous chunk's stores have read it
+            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const uint32_t at = ebuf + (uint32_t)lane * 64u + (uint32_t)((u ^ ((lane >> 1) & 3)) * 16);
+              sts128u(at, hi[4 * u], hi[4 * u + 1], hi[4 * u + 2], hi[4 * u + 3]);
+              sts128u(at + 2048u, lo[4 * u], lo[4 * u + 1], lo[4 * u + 2], lo[4 * u + 3]);
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&maps.d_hi, ebuf, nc, mq);
+              tma_store_2d(&maps.d_lo, ebuf + 2048u, nc, mq);
+              bulk_commit();
+            }
+            if (p.colsum_part) {
               const float s = warp_colsum32(v, lane);
-              if (nb + 32 * c + lane < p.N) p.colsum_part[(int64_t)(mq >> 5) * p.N + nb + 32 * c + lane] = s;
+              if (nc + lane < p.N) p.colsum_part[(int64_t)(mq >> 5) * p.N + nc + lane] = s;
             }
           }
         }
@@ -515,13 +542,15 @@ int launch_half_split(const float *x, int64_t rows, int64_t cols, int64_t ld, co
 }
 
 // ---------------------------------------------------------------------------------------- host side
-// Tensor map of a row-major [outer, inner] array: fp16 boxes with the 128-byte swizzle (64 elements
-// wide) for operands and d, fp32 boxes of [32][32] for C. Elements outside read as zero and are not written.
-static int make_map_16(CUtensorMap *map, const void *base, int64_t inner, int64_t outer, int64_t ld, int box_outer) {
+// Tensor map of a row-major [outer, inner] array: fp16 boxes of 64 elements with the 128-byte
+// swizzle for operands, of 32 with the 64-byte one for d, fp32 boxes of [32][32] for C. Elements outside read as zero and are not written.
+static int make_map_16(CUtensorMap *map, const void *base, int64_t inner, int64_t outer, int64_t ld, int box_outer,
+                       int box_inner = 64) {
   cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer}, strides[1] = {(cuuint64_t)ld * 2};
-  cuuint32_t box[2] = {64u, (cuuint32_t)box_outer}, estr[2] = {1u, 1u};
+  cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer}, estr[2] = {1u, 1u};
   const CUresult r = encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(base), dims, strides, box, estr,
-                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                 box_inner == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   EB_REQUIRE(r == CUDA_SUCCESS, ENDIA_B200_ECUDA, "fp16-pair product: cuTensorMapEncodeTiled failed with code %d", (int)r);
   return ENDIA_B200_OK;
@@ -611,8 +640,8 @@ int launch_gemm_f16(const F16Gemm &g, bool a_mn, bool b_mn, int epilogue, cudaSt
   if (epilogue == F16_STATS) {
     if (!a_mn && b_mn && !exact_a) return launch_kernel<false, true, 3, F16_STATS>(maps, p, s);
   } else if (epilogue == F16_DLOGITS) {
-    if ((st = make_map_16(&maps.d_hi, g.d_hi, g.N, g.M, g.ld_d, 32))) return st;
-    if ((st = make_map_16(&maps.d_lo, g.d_lo, g.N, g.M, g.ld_d, 32))) return st;
+    if ((st = make_map_16(&maps.d_hi, g.d_hi, g.N, g.M, g.ld_d, 32, 32))) return st;
+    if ((st = make_map_16(&maps.d_lo, g.d_lo, g.N, g.M, g.ld_d, 32, 32))) return st;
     if (!a_mn && b_mn && !exact_a) return launch_kernel<false, true, 3, F16_DLOGITS>(maps, p, s);
   } else {
     const int sp = g.partial ? k_ranges(g.M, g.N, g.K) : 1;

@@ -20,8 +20,8 @@ struct HalfPair {
 
 enum F16Epilogue {
   F16_STORE = 0,     // C = act(v + bias) or C += v
-  F16_STATS = 1,     // per row and 128 columns: max and sum of exp; the target's logit
-  F16_DLOGITS = 2    // d = (exp(v + bias - lse) - [column == target]) * coef, stored as an fp16 pair scaled by 2^15
+  F16_STATS = 1,     // per row and 128 columns: (max, sum of 2^(l - max)) of l = (v + bias) log2 e; the target's l
+  F16_DLOGITS = 2    // d = (2^((v + bias) log2 e - lse) - [column == target]) * coef, stored as an fp16 pair scaled by 2^15
 };
 constexpr float F16_D_SCALE = 32768.f;
 
@@ -40,11 +40,11 @@ struct F16Gemm {
   const float *target = nullptr;      // [M] class numbers; this product's columns are classes n_base ...
   int64_t n_base = 0;                 // (a multiple of 256)
   float2 *stats = nullptr;            // F16_STATS: [2 * ceil(V / 256)][M] (max, sum)
-  float *target_logit = nullptr;      // F16_STATS: [M]
-  const float *lse = nullptr, *coef = nullptr;   // F16_DLOGITS: [M]
+  float *target_logit = nullptr;      // F16_STATS: [M], in units of log2 e too
+  const float *lse = nullptr, *coef = nullptr;   // F16_DLOGITS: [M]; lse in units of log2 e
   __half *d_hi = nullptr, *d_lo = nullptr;       // F16_DLOGITS: [M][ld_d]
   int64_t ld_d = 0;
-  float *colsum_part = nullptr;       // F16_DLOGITS, optional: [ceil(M / 32)][N] sums over 32 rows of d (without the 2^15)
+  float *colsum_part = nullptr;       // F16_DLOGITS, optional: [ceil(M / 32)][N] sums over 32 rows of d (times 2^15)
 };
 
 // C[M, N] = A B: a_mn = false: A is stored [M, K]; true: [K, M].  b_mn = true: B is stored [K, N]; false: [N, K].

@@ -18,7 +18,9 @@ using namespace eb;
 
 namespace eb {
 
-// state: [0] rows that count, [1] and [2] the scales' maxima of x and W (bits), [4 ...) lse per row
+// state: [0] rows that count, [1] and [2] the scales' maxima of x and W (bits), [4 ...) lse per row, then
+// lse log2 e per row. Inside, logits are in units of log2 e: exponentials are powers of two.
+constexpr double CE_LOG2E = 1.4426950408889634, CE_LN2 = 0.6931471805599453;
 constexpr int CE_STATE_HEAD = 4;
 // Work space for one piece of the vocabulary (the d pair and W's pair, 4 bytes each per element).
 constexpr int64_t CE_PIECE_BYTES = (int64_t)256 << 20;
@@ -32,7 +34,8 @@ __device__ __forceinline__ bool ce_invalid(float t, int V) { return !(t < (float
 // Rows of a CTA: 32; its 16 warps take the parts of a row's (max, sum) in turn, lanes along the rows.
 __global__ void __launch_bounds__(512)
 ce_rows_kernel(const float2 *__restrict__ stats, int parts, const float *__restrict__ target,
-               const float *__restrict__ target_logit, int M, int V, float *__restrict__ lse, float *__restrict__ row_loss) {
+               const float *__restrict__ target_logit, int M, int V, float *__restrict__ lse, float *__restrict__ lse2,
+               float *__restrict__ row_loss) {
   __shared__ float2 part[16][32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int m = (int)blockIdx.x * 32 + lane;
@@ -45,7 +48,7 @@ ce_rows_kernel(const float2 *__restrict__ stats, int parts, const float *__restr
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const float nm = fmaxf(mx, v[u].x);
-        if (nm > -INFINITY) sum = sum * expf(mx - nm) + v[u].y * expf(v[u].x - nm);
+        if (nm > -INFINITY) sum = sum * exp2f(mx - nm) + v[u].y * exp2f(v[u].x - nm);
         else sum += v[u].y;      // (0, or NaN)
         mx = nm;
       }
@@ -57,14 +60,15 @@ ce_rows_kernel(const float2 *__restrict__ stats, int parts, const float *__restr
     for (int i = 1; i < 16; ++i) {
       const float2 v = part[i][lane];
       const float nm = fmaxf(mx, v.x);
-      if (nm > -INFINITY) sum = sum * expf(mx - nm) + v.y * expf(v.x - nm);
+      if (nm > -INFINITY) sum = sum * exp2f(mx - nm) + v.y * exp2f(v.x - nm);
       else sum += v.y;
       mx = nm;
     }
     const float t = __ldg(target + m);
-    const float l = mx + logf(sum);
-    lse[m] = l;
-    row_loss[m] = t < 0.f ? 0.f : (ce_invalid(t, V) ? NAN : l - target_logit[m]);
+    const double l2 = (double)mx + (double)log2f(sum);
+    lse[m] = (float)(l2 * CE_LN2);
+    lse2[m] = (float)l2;
+    row_loss[m] = t < 0.f ? 0.f : (ce_invalid(t, V) ? NAN : (float)((l2 - (double)target_logit[m]) * CE_LN2));
   }
 }
 
@@ -170,7 +174,7 @@ ce_piece_stats_kernel(const float *__restrict__ l, int64_t ld, int N, int n_base
   for (int m = (int)blockIdx.x; m < M; m += (int)gridDim.x) {
     const float *row = l + (int64_t)m * ld;
     float mx = -INFINITY;
-    for (int n = threadIdx.x; n < N; n += 256) mx = fmaxf(mx, row[n]);
+    for (int n = threadIdx.x; n < N; n += 256) mx = fmaxf(mx, row[n] * (float)CE_LOG2E);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     __syncthreads();
@@ -180,8 +184,8 @@ ce_piece_stats_kernel(const float *__restrict__ l, int64_t ld, int N, int n_base
     for (int i = 0; i < 8; ++i) mx = fmaxf(mx, sh[i]);
     float s = 0.f;
     for (int n = threadIdx.x; n < N; n += 256) {
-      const float v = row[n];
-      s += v == -INFINITY ? 0.f : expf(v - mx);
+      const float v = row[n] * (float)CE_LOG2E;
+      s += v == -INFINITY ? 0.f : exp2f(v - mx);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -193,7 +197,7 @@ ce_piece_stats_kernel(const float *__restrict__ l, int64_t ld, int N, int n_base
       for (int i = 0; i < 8; ++i) s += sh[i];
       stats[m] = make_float2(mx, s);
       const float t = target[m];
-      if (t >= (float)n_base && t < (float)(n_base + N)) target_logit[m] = row[(int)t - n_base];
+      if (t >= (float)n_base && t < (float)(n_base + N)) target_logit[m] = row[(int)t - n_base] * (float)CE_LOG2E;
     }
   }
 }
@@ -206,7 +210,7 @@ ce_piece_d_kernel(float *__restrict__ l, int64_t ld, int N, int n_base, const fl
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
     const int m = (int)(i / N), n = (int)(i - (int64_t)m * N);
     const float c = coef[m];
-    const float e = expf(l[(int64_t)m * ld + n] - lse[m]) - (target[m] == (float)(n_base + n) ? 1.f : 0.f);
+    const float e = exp2f(l[(int64_t)m * ld + n] * (float)CE_LOG2E - lse[m]) - (target[m] == (float)(n_base + n) ? 1.f : 0.f);
     l[(int64_t)m * ld + n] = c == 0.f ? 0.f : e * (c * __ldg(alpha));
   }
 }
@@ -313,7 +317,7 @@ static int ce_check(const float *x, int64_t ldx, const float *W, int64_t ldw, co
 
 extern "C" {
 
-size_t endia_b200_linear_ce_state_bytes(int64_t M) { return M < 0 ? 0 : sizeof(float) * (size_t)(CE_STATE_HEAD + M); }
+size_t endia_b200_linear_ce_state_bytes(int64_t M) { return M < 0 ? 0 : sizeof(float) * (size_t)(CE_STATE_HEAD + 2 * M); }
 
 size_t endia_b200_linear_ce_scratch_bytes(int64_t M, int64_t K, int64_t V, int32_t backward) {
   if (M <= 0 || K <= 0 || V <= 0 || V > CE_MAX_CLASSES || M > (1 << 27) || K > (1 << 27)) return 256;
@@ -365,7 +369,7 @@ int endia_b200_linear_ce_fwd(const float *x, int64_t ldx, const float *W, int64_
     }
   }
   ce_rows_kernel<<<(unsigned)ceil_div(M, 32), 512, 0, s>>>(f.stats, (int)f.parts, target, f.tl, (int)M, (int)V,
-                                                           state + CE_STATE_HEAD, rows);
+                                                           state + CE_STATE_HEAD, state + CE_STATE_HEAD + M, rows);
   EB_LAUNCH_CHECK();
   ce_loss_kernel<<<1, 1024, 0, s>>>(rows, target, (int)M, reduction == ENDIA_B200_LOSS_MEAN,
                                     reduction == ENDIA_B200_LOSS_NONE ? nullptr : loss, state);
@@ -389,7 +393,7 @@ int endia_b200_linear_ce_bwd(const float *x, int64_t ldx, const float *W, int64_
   }
   CeBackward f;
   ce_carve_backward(M, K, V, static_cast<char *>(scratch), f);
-  const float *lse = state + CE_STATE_HEAD;
+  const float *lse = state + CE_STATE_HEAD + M;      // (in units of log2 e)
   const uint32_t *amax = reinterpret_cast<const uint32_t *>(state) + 1;
   const bool small = ce_small(M, K, V, true);
   ce_coef_kernel<<<1, 1024, 0, s>>>(grad, reduction == ENDIA_B200_LOSS_NONE, reduction == ENDIA_B200_LOSS_MEAN, state, target,
@@ -453,7 +457,7 @@ int endia_b200_linear_ce_bwd(const float *x, int64_t ldx, const float *W, int64_
       if ((st = launch_gemm_f16(h, true, true, F16_STORE, s))) return st;
     }
     if (db) {
-      ce_db_kernel<<<(unsigned)ceil_div(n, 32), 256, 0, s>>>(f.part_sums, (int)ceil_div(M, 32), (int)n, f.alpha, db + v0);
+      ce_db_kernel<<<(unsigned)ceil_div(n, 32), 256, 0, s>>>(f.part_sums, (int)ceil_div(M, 32), (int)n, f.alpha + 1, db + v0);
       EB_LAUNCH_CHECK();
     }
   }
