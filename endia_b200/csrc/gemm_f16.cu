@@ -448,29 +448,75 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
   }
 }
 
-// C = act(sum over the ranges of K, in order, unscaled, + bias), or C += it.
+// C = act(sum over the ranges of K, in order, unscaled, + bias), or C += it. Four consecutive columns per
+// thread (the rows of the work space are 16-byte aligned).
 __global__ void __launch_bounds__(256)
 gemm_f16_finish_kernel(const F16Params p, const float *__restrict__ partial, int64_t ld_partial, int64_t slice, int parts) {
   const float f0 = half_unscale(p.amax_a);
   const float f1 = half_unscale(p.amax_b) * (p.alpha_dev ? __ldg(p.alpha_dev) : 1.f);
-  const int n = (int)(blockIdx.x * blockDim.x + threadIdx.x);
-  if (n >= p.N) return;
-  const float bv = p.bias ? __ldg(p.bias + n) : 0.f;
-  for (int m = (int)blockIdx.y; m < p.M; m += (int)gridDim.y) {
-    const float *src = partial + (int64_t)m * ld_partial + n;
-    float v = 0.f;
-    for (int s0 = 0; s0 < parts; s0 += 8) {
-      float t[8];
+  const uint32_t per_row = (uint32_t)((p.N + 3) / 4);
+  const int64_t total = (int64_t)p.M * per_row, step = (int64_t)gridDim.x * blockDim.x;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
+    const int64_t m = total < ((int64_t)1 << 31) ? (int64_t)((uint32_t)i / per_row) : i / per_row;
+    const int n = (int)(i - m * per_row) * 4;
+    const float *src = partial + m * ld_partial + n;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < parts; s0 += 4) {
+      float4 t[4];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) t[u] = s0 + u < parts ? __ldcs(src + (int64_t)(s0 + u) * slice) : 0.f;
+      for (int u = 0; u < 4; ++u)
+        t[u] = s0 + u < parts ? __ldcs(reinterpret_cast<const float4 *>(src + (int64_t)(s0 + u) * slice)) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int u = 0; u < 8; ++u) v += t[u];
+      for (int u = 0; u < 4; ++u) { v[0] += t[u].x; v[1] += t[u].y; v[2] += t[u].z; v[3] += t[u].w; }
     }
-    v = (v * f0) * f1 + bv;
-    if (p.act) v = act_fwd(p.act, v);
-    float *c = p.C + (int64_t)m * p.ldc + n;
-    *c = p.accumulate ? *c + v : v;
+    float *c = p.C + m * p.ldc + n;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (n + k < p.N) {
+        v[k] = (v[k] * f0) * f1 + (p.bias ? __ldg(p.bias + n + k) : 0.f);
+        if (p.act) v[k] = act_fwd(p.act, v[k]);
+        if (p.accumulate) v[k] += c[k];
+      }
+    }
+    if (p.vec_c && n + 4 <= p.N) {
+      *reinterpret_cast<float4 *>(c) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (n + k < p.N) c[k] = v[k];
+    }
   }
+}
+
+// out[n] = alpha * sum over the parts [parts][N], in a fixed order: 32 columns per CTA, its eight warps take
+// the parts in turn with eight loads in flight.
+__global__ void __launch_bounds__(256)
+column_sums_kernel(const float *__restrict__ part, int parts, int64_t N, const float *__restrict__ alpha, float *__restrict__ out) {
+  __shared__ float sh[8][33];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t n = (int64_t)blockIdx.x * 32 + lane;
+  float s = 0.f;
+  if (n < N) {
+    for (int r0 = w; r0 < parts; r0 += 64) {
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = r0 + 8 * u < parts ? __ldg(part + (int64_t)(r0 + 8 * u) * N + n) : 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += v[u];
+    }
+  }
+  sh[w][lane] = s;
+  __syncthreads();
+  if (w == 0 && n < N) {
+    for (int i = 1; i < 8; ++i) s += sh[i][lane];
+    out[n] = alpha ? s * __ldg(alpha) : s;
+  }
+}
+
+int launch_column_sums(const float *part, int parts, int64_t N, const float *alpha, float *out, cudaStream_t s) {
+  column_sums_kernel<<<(unsigned)ceil_div(N, 32), 256, 0, s>>>(part, parts, N, alpha, out);
+  EB_LAUNCH_CHECK();
+  return ENDIA_B200_OK;
 }
 
 // ---------------------------------------------------------------------------- passes over fp32 arrays
@@ -680,8 +726,7 @@ int launch_gemm_f16(const F16Gemm &g, bool a_mn, bool b_mn, int epilogue, cudaSt
     else if (a_mn && b_mn) st = launch_kernel<true, true, 2, F16_STORE>(maps, p, s);
     else { set_error("fp16-pair product: no kernel for these layouts"); return ENDIA_B200_EINVAL; }
     if (st || sp < 2) return st;
-    const dim3 grid((unsigned)ceil_div(g.N, 256), (unsigned)(g.M < 1024 ? g.M : 1024));
-    gemm_f16_finish_kernel<<<grid, 256, 0, s>>>(p, g.partial, ldp, (int64_t)p.part_rows * ldp, sp);
+    gemm_f16_finish_kernel<<<grid_for(g.M * ceil_div(g.N, 4), 256), 256, 0, s>>>(p, g.partial, ldp, (int64_t)p.part_rows * ldp, sp);
     EB_LAUNCH_CHECK();
     return ENDIA_B200_OK;
   }

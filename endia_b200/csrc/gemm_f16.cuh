@@ -61,6 +61,9 @@ int launch_amax(const float *x, int64_t rows, int64_t cols, int64_t ld, const fl
 int launch_half_split(const float *x, int64_t rows, int64_t cols, int64_t ld, const float *target,
                       const uint32_t *amax, __half *hi, __half *lo, int64_t ld_out, cudaStream_t s);
 
+// out[n] = alpha (a device scalar, NULL: 1) times the sum of the rows of part [parts][N], in a fixed order.
+int launch_column_sums(const float *part, int parts, int64_t N, const float *alpha, float *out, cudaStream_t s);
+
 // C = act(A B + bias) + beta C on the fp32 kernels (row-major; ta / tb: stored transposed).
 int gemm_fp32(int ta, int tb, int64_t M, int64_t N, int64_t K, const float *A, int64_t lda, const float *B, int64_t ldb,
               float *C, int64_t ldc, const float *bias, int act, float beta, cudaStream_t s);

@@ -39,55 +39,66 @@ __host__ __device__ static inline Kept kept_view(void *p, int64_t rows, int64_t 
   return k;
 }
 
-// 8 lanes per block of 32, four values each (128-bit loads where VEC).
+// 4 lanes per block of 32, eight values each (128-bit loads where VEC); two blocks per lane group in flight.
+template <bool VEC>
+__device__ __forceinline__ void keep_load(const float *src, int64_t left, float (&v)[8]) {
+  if (VEC && left >= 8) {
+    const float4 a = __ldg(reinterpret_cast<const float4 *>(src)), b = __ldg(reinterpret_cast<const float4 *>(src) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = u < left ? __ldg(src + u) : 0.f;
+  }
+}
 template <bool VEC>
 __global__ void __launch_bounds__(256)
 keep8_kernel(const float *__restrict__ x, int64_t ld, int64_t rows, int64_t cols, int keep_sign, Kept k) {
-  const int64_t per_row = k.ldq / 4, total = rows * per_row, step = (int64_t)gridDim.x * blockDim.x;
+  constexpr int IN_FLIGHT = 2;
+  const int64_t per_row = k.ldq / 8, total = rows * per_row, step = (int64_t)gridDim.x * blockDim.x;
   const bool narrow = total < ((int64_t)1 << 31);
   uint32_t best = 0;
-  // (whole warps take part in the exchanges: total is a multiple of 8, the tail of a warp idles along)
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i - (threadIdx.x & 31) < total; i += step) {
-    const bool in = i < total;
-    const int64_t r = !in ? 0 : (narrow ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row);
-    const int64_t c = in ? (i - r * per_row) * 4 : 0, left = in ? cols - c : 0;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    const float *src = x + r * ld + c;
-    if (VEC && left >= 4) {
-      const float4 t = __ldg(reinterpret_cast<const float4 *>(src));
-      v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
-    } else {
+  // (total is a multiple of 4 and whole warps stay in the loop, so that the exchanges have all their lanes)
+  for (int64_t i0 = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i0 - (threadIdx.x & 31) < total; i0 += IN_FLIGHT * step) {
+    float v[IN_FLIGHT][8];
+    int64_t row[IN_FLIGHT], col[IN_FLIGHT];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) if (u < left) v[u] = __ldg(src + u);
-    }
-    uint32_t mx = 0;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const uint32_t b = __float_as_uint(v[u]) & 0x7FFFFFFFu;
-      if (b < 0x7F800000u && b > mx) mx = b;
+    for (int f = 0; f < IN_FLIGHT; ++f) {
+      const int64_t i = i0 + f * step;
+      const bool in = i < total;
+      row[f] = !in ? -1 : (narrow ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row);
+      col[f] = in ? (i - row[f] * per_row) * 8 : 0;
+      keep_load<VEC>(x + (in ? row[f] * ld : 0) + col[f], in ? cols - col[f] : 0, v[f]);
     }
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) {
-      const uint32_t b = __shfl_xor_sync(0xffffffffu, mx, o);
-      mx = b > mx ? b : mx;
-    }
-    best = mx > best ? mx : best;
-    // max / 2^e < 127.5: 127.5 = 64 * 1.9921875
-    int e = (int)(mx >> 23) - 127 - 6 + ((mx & 0x7FFFFFu) >= 0x7F0000u ? 1 : 0);
-    e = e < -126 ? -126 : e;
-    const float down = pow2f_exact(-e);
-    char4 q;
-    int8_t *qp = reinterpret_cast<int8_t *>(&q);
+    for (int f = 0; f < IN_FLIGHT; ++f) {
+      uint32_t mx = 0;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const uint32_t b = __float_as_uint(v[u]) & 0x7FFFFFFFu;
-      int n = b < 0x7F800000u ? __float2int_rn(v[u] * down) : -128;
-      if (keep_sign && n == 0 && b != 0) n = v[u] < 0.f ? -1 : 1;
-      qp[u] = (int8_t)n;
-    }
-    if (in) {
-      *reinterpret_cast<char4 *>(k.q + r * k.ldq + c) = q;
-      if ((threadIdx.x & 7) == 0) k.e[r * k.lde + c / 32] = (uint8_t)(e + 127);
+      for (int u = 0; u < 8; ++u) {
+        const uint32_t b = __float_as_uint(v[f][u]) & 0x7FFFFFFFu;
+        if (b < 0x7F800000u && b > mx) mx = b;
+      }
+#pragma unroll
+      for (int o = 2; o > 0; o >>= 1) {
+        const uint32_t b = __shfl_xor_sync(0xffffffffu, mx, o);
+        mx = b > mx ? b : mx;
+      }
+      best = mx > best ? mx : best;
+      // max / 2^e < 127.5: 127.5 = 64 * 1.9921875
+      int e = (int)(mx >> 23) - 127 - 6 + ((mx & 0x7FFFFFu) >= 0x7F0000u ? 1 : 0);
+      e = e < -126 ? -126 : e;
+      const float down = pow2f_exact(-e);
+      uint32_t w[2] = {0u, 0u};
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const uint32_t b = __float_as_uint(v[f][u]) & 0x7FFFFFFFu;
+        int n = b < 0x7F800000u ? __float2int_rn(v[f][u] * down) : -128;
+        if (keep_sign && n == 0 && b != 0) n = v[f][u] < 0.f ? -1 : 1;
+        w[u >> 2] |= ((uint32_t)n & 0xFFu) << (8 * (u & 3));
+      }
+      if (row[f] >= 0) {
+        *reinterpret_cast<uint2 *>(k.q + row[f] * k.ldq + col[f]) = make_uint2(w[0], w[1]);
+        if ((threadIdx.x & 3) == 0) k.e[row[f] * k.lde + col[f] / 32] = (uint8_t)(e + 127);
+      }
     }
   }
   best = __reduce_max_sync(0xffffffffu, best);
@@ -125,20 +136,26 @@ kept_read_kernel(Kept k, int64_t rows, int64_t cols, float *__restrict__ out) {
 }
 
 // The kept values as one fp16 operand (exact: q has 7 bits; values below 2^-24 of the array's scale
-// step, 2^-38 of its largest value, round to nothing).
+// step, 2^-38 of its largest value, round to nothing). Sixteen values per thread.
 __global__ void __launch_bounds__(256)
 kept_half_kernel(Kept k, int64_t rows, __half *__restrict__ out) {
-  const int64_t per_row = k.ldq / 8, total = rows * per_row, step = (int64_t)gridDim.x * blockDim.x;
+  const int64_t per_row = k.ldq / 16, total = rows * per_row, step = (int64_t)gridDim.x * blockDim.x;
   const bool narrow = total < ((int64_t)1 << 31);
   const float s = half_scale(k.amax);
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
-    const int64_t r = narrow ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row, c = (i - r * per_row) * 8;
-    float v[8];
-    kept8(k, r, c, s, v);
-    __half h[8];
+    const int64_t r = narrow ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row, c = (i - r * per_row) * 16;
+    const uint4 w = __ldg(reinterpret_cast<const uint4 *>(k.q + r * k.ldq + c));
+    const float unit = pow2f_exact((int)__ldg(k.e + r * k.lde + c / 32) - 127);
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+    __half h[16];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) h[u] = __float2half_rn(v[u]);
-    *reinterpret_cast<uint4 *>(out + r * k.ldq + c) = *reinterpret_cast<uint4 *>(h);
+    for (int u = 0; u < 16; ++u) {
+      const int n = (int)(int8_t)((ws[u >> 2] >> (8 * (u & 3))) & 0xFFu);
+      h[u] = __float2half_rn(n == -128 ? NAN : ((float)n * unit) * s);
+    }
+    uint4 *dst = reinterpret_cast<uint4 *>(out + r * k.ldq + c);
+    dst[0] = reinterpret_cast<uint4 *>(h)[0];
+    dst[1] = reinterpret_cast<uint4 *>(h)[1];
   }
 }
 
@@ -288,7 +305,7 @@ static int run_keep8(const float *x, int64_t ld, int64_t rows, int64_t cols, int
   EB_CUDA(cudaMemsetAsync(kept, 0, 256, s));
   if (rows == 0 || cols == 0) return ENDIA_B200_OK;
   const Kept k = kept_view(kept, rows, cols);
-  const int grid = grid_for(rows * (k.ldq / 4), 256, 8);
+  const int grid = grid_for(rows * (k.ldq / 8), 256, 8);
   const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ld % 4 == 0 || rows == 1);
   if (vec) keep8_kernel<true><<<grid, 256, 0, s>>>(x, ld, rows, cols, keep_sign, k);
   else keep8_kernel<false><<<grid, 256, 0, s>>>(x, ld, rows, cols, keep_sign, k);
@@ -352,13 +369,15 @@ int endia_b200_linear_keep_fwd(const float *x, int64_t ldx, const float *W, int6
   KeepForward f;
   keep_carve_forward(M, N, K, static_cast<char *>(scratch), f);
   EB_CUDA(cudaMemsetAsync(f.amax, 0, 2 * sizeof(uint32_t), s));
-  if ((st = launch_amax(x, M, K, ldx, nullptr, f.amax, s))) return st;
+  // the 8-bit form has found the largest |x| already
+  const uint32_t *amax_x = kept_x ? static_cast<const uint32_t *>(kept_x) : f.amax;
+  if (!kept_x && (st = launch_amax(x, M, K, ldx, nullptr, f.amax, s))) return st;
   if ((st = launch_amax(W, K, N, ldw, nullptr, f.amax + 1, s))) return st;
-  if ((st = launch_half_split(x, M, K, ldx, nullptr, f.amax, f.xh, f.xl, f.ldx, s))) return st;
+  if ((st = launch_half_split(x, M, K, ldx, nullptr, amax_x, f.xh, f.xl, f.ldx, s))) return st;
   if ((st = launch_half_split(W, K, N, ldw, nullptr, f.amax + 1, f.wh, f.wl, f.ldw, s))) return st;
   F16Gemm g;
   g.M = M; g.N = N; g.K = K;
-  g.a = HalfPair{f.xh, f.xl, f.ldx, f.amax};
+  g.a = HalfPair{f.xh, f.xl, f.ldx, amax_x};
   g.b = HalfPair{f.wh, f.wl, f.ldw, f.amax + 1};
   g.bias = bias; g.act = act; g.C = out; g.ldc = N; g.partial = f.partial;
   return launch_gemm_f16(g, false, true, F16_STORE, s);
@@ -396,7 +415,7 @@ int endia_b200_linear_keep_bwd(const void *kept_x, const float *W, int64_t ldw, 
   }
   ds_split_kernel<<<grid, 256, 0, s>>>(a, f.amax, f.dh, f.dl, f.ldd, f.ds32, db ? f.sums : nullptr);
   EB_LAUNCH_CHECK();
-  if (db && (st = launch_colsum_finish(f.sums, db, N, (int)ceil_div(M, 64), 1, s))) return st;
+  if (db && (st = launch_column_sums(f.sums, (int)ceil_div(M, 64), N, nullptr, db, s))) return st;
   const Kept kx = kept_view(const_cast<void *>(kept_x), M, K);
   if (small) {
     if (dx && (st = gemm_fp32(0, 1, M, K, N, f.ds32, N, W, ldw, dx, K, nullptr, 0, 0.f, s))) return st;
@@ -409,7 +428,7 @@ int endia_b200_linear_keep_bwd(const void *kept_x, const float *W, int64_t ldw, 
   }
   const HalfPair d{f.dh, f.dl, f.ldd, f.amax};
   if (dw) {
-    kept_half_kernel<<<grid_for(M * (kx.ldq / 8), 256, 8), 256, 0, s>>>(kx, M, f.x8);
+    kept_half_kernel<<<grid_for(M * (kx.ldq / 16), 256, 8), 256, 0, s>>>(kx, M, f.x8);
     EB_LAUNCH_CHECK();
     F16Gemm g;
     g.M = K; g.N = N; g.K = M;

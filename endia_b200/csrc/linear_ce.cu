@@ -140,30 +140,6 @@ ce_coef_kernel(const float *__restrict__ g, int per_row, int mean, const float *
   }
 }
 
-// db[v] = alpha * sum over the parts, in order.
-__global__ void __launch_bounds__(256)
-ce_db_kernel(const float *__restrict__ part, int parts, int N, const float *__restrict__ alpha, float *__restrict__ db) {
-  __shared__ float sh[8][33];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int n = (int)blockIdx.x * 32 + lane;
-  float s = 0.f;
-  if (n < N) {
-    for (int r0 = w; r0 < parts; r0 += 64) {
-      float v[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = r0 + 8 * u < parts ? __ldg(part + (int64_t)(r0 + 8 * u) * N + n) : 0.f;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) s += v[u];
-    }
-  }
-  sh[w][lane] = s;
-  __syncthreads();
-  if (w == 0 && n < N) {
-    for (int i = 1; i < 8; ++i) s += sh[i][lane];
-    db[n] = s * __ldg(alpha);
-  }
-}
-
 // ------------------------------------------------------------------------------------ small problems, fp32
 // (max, sum) and the target's logit of one row of a piece; one CTA per row.
 __global__ void __launch_bounds__(256)
@@ -456,10 +432,7 @@ int endia_b200_linear_ce_bwd(const float *x, int64_t ldx, const float *W, int64_
       h.C = dw + v0; h.ldc = V; h.partial = f.partial;
       if ((st = launch_gemm_f16(h, true, true, F16_STORE, s))) return st;
     }
-    if (db) {
-      ce_db_kernel<<<(unsigned)ceil_div(n, 32), 256, 0, s>>>(f.part_sums, (int)ceil_div(M, 32), (int)n, f.alpha + 1, db + v0);
-      EB_LAUNCH_CHECK();
-    }
+    if (db && (st = launch_column_sums(f.part_sums, (int)ceil_div(M, 32), n, f.alpha + 1, db + v0, s))) return st;
   }
   return ENDIA_B200_OK;
 }
