@@ -520,10 +520,15 @@ int launch_column_sums(const float *part, int parts, int64_t N, const float *alp
 }
 
 // ---------------------------------------------------------------------------- passes over fp32 arrays
-// Eight consecutive columns per thread; VEC: 128-bit loads (leading dimension and base allow them).
-template <bool VEC>
-__device__ __forceinline__ void load8(const float *src, int64_t left, float (&v)[8]) {
-  if (VEC && left >= 8) {
+// Eight consecutive columns per thread; vec: 128-bit loads (leading dimension and base allow them). CTAs
+// [0, split) work on the first array, the others on the second.
+struct HalfJobs {
+  HalfJob job[2];
+  bool vec[2];
+  int split;
+};
+__device__ __forceinline__ void load8(const float *src, int64_t left, bool vec, float (&v)[8]) {
+  if (vec && left >= 8) {
     const float4 a = __ldg(reinterpret_cast<const float4 *>(src)), b = __ldg(reinterpret_cast<const float4 *>(src) + 1);
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   } else {
@@ -531,78 +536,87 @@ __device__ __forceinline__ void load8(const float *src, int64_t left, float (&v)
     for (int i = 0; i < 8; ++i) v[i] = i < left ? __ldg(src + i) : 0.f;
   }
 }
-__device__ __forceinline__ void row_and_col(int64_t i, int64_t per_row, bool narrow, int64_t &r, int64_t &c) {
-  r = narrow ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row;
-  c = i - r * per_row;
+template <typename F>
+__device__ __forceinline__ void for_groups_of_8(const HalfJobs &jobs, F f) {
+  const bool second = (int)blockIdx.x >= jobs.split;
+  const HalfJob &j = jobs.job[second ? 1 : 0];
+  const bool vec = jobs.vec[second ? 1 : 0];
+  const int block = (int)blockIdx.x - (second ? jobs.split : 0), blocks = second ? (int)gridDim.x - jobs.split : jobs.split;
+  const int64_t per_row = (j.cols + 7) / 8, total = j.rows * per_row, step = (int64_t)blocks * blockDim.x;
+  const bool narrow = total < ((int64_t)1 << 31);
+  for (int64_t i = (int64_t)block * blockDim.x + threadIdx.x; i < total; i += step) {
+    const int64_t r = narrow ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row, c = (i - r * per_row) * 8;
+    f(j, vec, r, c);
+  }
 }
 
-template <bool VEC>
-__global__ void __launch_bounds__(256)
-amax_kernel(const float *__restrict__ x, int64_t rows, int64_t cols, int64_t ld, const float *__restrict__ target,
-            uint32_t *__restrict__ amax) {
-  const int64_t per_row = (cols + 7) / 8, total = rows * per_row, step = (int64_t)gridDim.x * blockDim.x;
-  const bool narrow = total < ((int64_t)1 << 31);
+__global__ void __launch_bounds__(256) amax_kernel(const __grid_constant__ HalfJobs jobs) {
   uint32_t best = 0;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
-    int64_t r, c;
-    row_and_col(i, per_row, narrow, r, c);
-    if (target && __ldg(target + r) < 0.f) continue;
+  for_groups_of_8(jobs, [&](const HalfJob &j, bool vec, int64_t r, int64_t c) {
+    if (j.target && __ldg(j.target + r) < 0.f) return;
     float v[8];
-    load8<VEC>(x + r * ld + c * 8, cols - c * 8, v);
+    load8(j.x + r * j.ld + c, j.cols - c, vec, v);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const uint32_t b = __float_as_uint(v[k]) & 0x7FFFFFFFu;
       if (b < 0x7F800000u && b > best) best = b;
     }
-  }
+  });
   best = __reduce_max_sync(0xffffffffu, best);
-  if ((threadIdx.x & 31) == 0 && best) atomicMax(amax, best);   // (a maximum: any order gives the same bits)
+  // (a maximum: any order gives the same bits)
+  if ((threadIdx.x & 31) == 0 && best) atomicMax(jobs.job[(int)blockIdx.x >= jobs.split ? 1 : 0].amax, best);
 }
 
-template <bool VEC>
-__global__ void __launch_bounds__(256)
-half_split_kernel(const float *__restrict__ x, int64_t rows, int64_t cols, int64_t ld, const float *__restrict__ target,
-                  const uint32_t *__restrict__ amax, __half *__restrict__ hi, __half *__restrict__ lo, int64_t ld_out) {
-  const int64_t per_row = (cols + 7) / 8, total = rows * per_row, step = (int64_t)gridDim.x * blockDim.x;
-  const bool narrow = total < ((int64_t)1 << 31);
-  const float s = half_scale(amax);
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
-    int64_t r, c;
-    row_and_col(i, per_row, narrow, r, c);
+__global__ void __launch_bounds__(256) half_split_kernel(const __grid_constant__ HalfJobs jobs) {
+  const float s = half_scale(jobs.job[(int)blockIdx.x >= jobs.split ? 1 : 0].amax);
+  for_groups_of_8(jobs, [&](const HalfJob &j, bool vec, int64_t r, int64_t c) {
     float v[8];
-    if (target && __ldg(target + r) < 0.f) {
+    if (j.target && __ldg(j.target + r) < 0.f) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = 0.f;
     } else {
-      load8<VEC>(x + r * ld + c * 8, cols - c * 8, v);
+      load8(j.x + r * j.ld + c, j.cols - c, vec, v);
     }
     __half h[8], l[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) half_pair(v[k] * s, h[k], l[k]);
-    *reinterpret_cast<uint4 *>(hi + r * ld_out + c * 8) = *reinterpret_cast<uint4 *>(h);   // (ld_out covers whole groups of 8)
-    *reinterpret_cast<uint4 *>(lo + r * ld_out + c * 8) = *reinterpret_cast<uint4 *>(l);
-  }
+    // (ld_out covers whole groups of 8)
+    *reinterpret_cast<uint4 *>(j.hi + r * j.ld_out + c) = *reinterpret_cast<uint4 *>(h);
+    *reinterpret_cast<uint4 *>(j.lo + r * j.ld_out + c) = *reinterpret_cast<uint4 *>(l);
+  });
 }
 
 static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-int launch_amax(const float *x, int64_t rows, int64_t cols, int64_t ld, const float *target, uint32_t *amax,
-                cudaStream_t s) {
-  if (rows <= 0 || cols <= 0) return ENDIA_B200_OK;
-  if (!target && ld == cols) { cols *= rows; ld = cols; rows = 1; }
-  const int grid = grid_for(rows * ceil_div(cols, 8), 256, 8);
-  if (aligned16(x) && (ld % 4 == 0 || rows == 1)) amax_kernel<true><<<grid, 256, 0, s>>>(x, rows, cols, ld, target, amax);
-  else amax_kernel<false><<<grid, 256, 0, s>>>(x, rows, cols, ld, target, amax);
+// Splits the grid of a pass by the arrays' sizes; 0 CTAs when there is nothing to do.
+static int plan_jobs(HalfJobs &jobs, const HalfJob &a, const HalfJob *b, bool flat) {
+  int64_t groups[2] = {0, 0};
+  for (int i = 0; i < 2; ++i) {
+    if (i == 1 && !b) break;
+    HalfJob &j = jobs.job[i] = i == 0 ? a : *b;
+    if (flat && !j.target && j.ld == j.cols) { j.cols *= j.rows; j.ld = j.cols; j.rows = j.cols > 0 ? 1 : 0; }
+    jobs.vec[i] = aligned16(j.x) && (j.ld % 4 == 0 || j.rows == 1);
+    groups[i] = j.rows * ceil_div(j.cols, 8);
+  }
+  const int g0 = groups[0] ? grid_for(groups[0], 256, 8) : 0, g1 = groups[1] ? grid_for(groups[1], 256, 8) : 0;
+  jobs.split = g0;
+  return g0 + g1;
+}
+
+int launch_amax(const HalfJob &a, const HalfJob *b, cudaStream_t s) {
+  HalfJobs jobs;
+  const int grid = plan_jobs(jobs, a, b, true);
+  if (grid == 0) return ENDIA_B200_OK;
+  amax_kernel<<<grid, 256, 0, s>>>(jobs);
   EB_LAUNCH_CHECK();
   return ENDIA_B200_OK;
 }
 
-int launch_half_split(const float *x, int64_t rows, int64_t cols, int64_t ld, const float *target,
-                      const uint32_t *amax, __half *hi, __half *lo, int64_t ld_out, cudaStream_t s) {
-  if (rows <= 0 || cols <= 0) return ENDIA_B200_OK;
-  const int grid = grid_for(rows * ceil_div(cols, 8), 256, 8);
-  if (aligned16(x) && (ld % 4 == 0 || rows == 1)) half_split_kernel<true><<<grid, 256, 0, s>>>(x, rows, cols, ld, target, amax, hi, lo, ld_out);
-  else half_split_kernel<false><<<grid, 256, 0, s>>>(x, rows, cols, ld, target, amax, hi, lo, ld_out);
+int launch_half_split(const HalfJob &a, const HalfJob *b, cudaStream_t s) {
+  HalfJobs jobs;
+  const int grid = plan_jobs(jobs, a, b, false);
+  if (grid == 0) return ENDIA_B200_OK;
+  half_split_kernel<<<grid, 256, 0, s>>>(jobs);
   EB_LAUNCH_CHECK();
   return ENDIA_B200_OK;
 }
@@ -732,18 +746,6 @@ int launch_gemm_f16(const F16Gemm &g, bool a_mn, bool b_mn, int epilogue, cudaSt
   }
   set_error("fp16-pair product: no kernel for these layouts");
   return ENDIA_B200_EINVAL;
-}
-
-int gemm_fp32(int ta, int tb, int64_t M, int64_t N, int64_t K, const float *A, int64_t lda, const float *B, int64_t ldb,
-              float *C, int64_t ldc, const float *bias, int act, float beta, cudaStream_t s) {
-  GemmParams p{};
-  p.A = A; p.B = B; p.C = C; p.M = M; p.N = N; p.K = K; p.lda = lda; p.ldb = ldb; p.ldc = ldc;
-  p.vec_a = aligned16(A) && lda % 4 == 0;
-  p.vec_b = aligned16(B) && ldb % 4 == 0;
-  p.vec_c = aligned16(C) && ldc % 4 == 0;
-  p.epi.alpha = 1.f; p.epi.beta = beta; p.epi.bias = bias; p.epi.act = act;
-  if (skinny_gemm_supported(p, tb, 1)) return launch_gemm_skinny(p, ta, tb, s);
-  return launch_gemm_ffma(p, ta, tb, 1, s);
 }
 
 int f16_status_and_clear(cudaStream_t s) {

@@ -53,20 +53,23 @@ int launch_gemm_f16(const F16Gemm &g, bool a_mn, bool b_mn, int epilogue, cudaSt
 size_t gemm_f16_partial_bytes(int64_t M, int64_t N, int64_t K);
 bool gemm_f16_available();
 
-// amax[0] = max(amax[0], bits of the largest finite |x|) over [rows, cols] (leading dimension ld);
-// `target` (optional, [rows]): rows with target < 0 are left out. amax must have been set to 0.
-int launch_amax(const float *x, int64_t rows, int64_t cols, int64_t ld, const float *target, uint32_t *amax,
-                cudaStream_t s);
-// The fp16 pair of x; rows with target < 0 become zero.
-int launch_half_split(const float *x, int64_t rows, int64_t cols, int64_t ld, const float *target,
-                      const uint32_t *amax, __half *hi, __half *lo, int64_t ld_out, cudaStream_t s);
+// One fp32 array of the passes below: [rows, cols], leading dimension ld. `target` (optional, [rows]):
+// rows with target < 0 do not count in the maximum and become zero in the pair.
+struct HalfJob {
+  const float *x = nullptr;
+  int64_t rows = 0, cols = 0, ld = 0;
+  const float *target = nullptr;
+  uint32_t *amax = nullptr;      // bits of the largest finite |x|
+  __half *hi = nullptr, *lo = nullptr;
+  int64_t ld_out = 0;
+};
+// amax[0] = max(amax[0], bits of the largest finite |x|) of up to two arrays in one launch; *amax starts at 0.
+int launch_amax(const HalfJob &a, const HalfJob *b, cudaStream_t s);
+// The fp16 pairs of up to two arrays in one launch.
+int launch_half_split(const HalfJob &a, const HalfJob *b, cudaStream_t s);
 
 // out[n] = alpha (a device scalar, NULL: 1) times the sum of the rows of part [parts][N], in a fixed order.
 int launch_column_sums(const float *part, int parts, int64_t N, const float *alpha, float *out, cudaStream_t s);
-
-// C = act(A B + bias) + beta C on the fp32 kernels (row-major; ta / tb: stored transposed).
-int gemm_fp32(int ta, int tb, int64_t M, int64_t N, int64_t K, const float *A, int64_t lda, const float *B, int64_t ldb,
-              float *C, int64_t ldc, const float *bias, int act, float beta, cudaStream_t s);
 
 struct Carver {       // a caller's work space, handed out in 256-byte steps (base NULL: only measures)
   char *base;

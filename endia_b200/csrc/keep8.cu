@@ -204,10 +204,10 @@ __global__ void __launch_bounds__(256) ds_amax_kernel(DsArgs a, uint32_t *__rest
   best = __reduce_max_sync(0xffffffffu, best);
   if ((threadIdx.x & 31) == 0 && best) atomicMax(amax, best);
 }
-// The fp16 pair of ds (or ds itself, ds32) and its sums over 64 rows: a CTA takes 64 rows x 128 columns.
+// The fp16 pair of ds and its sums over 64 rows: a CTA takes 64 rows x 128 columns.
 __global__ void __launch_bounds__(256)
 ds_split_kernel(DsArgs a, const uint32_t *__restrict__ amax, __half *__restrict__ hi, __half *__restrict__ lo, int64_t ld,
-                float *__restrict__ ds32, float *__restrict__ sums) {
+                float *__restrict__ sums) {
   __shared__ float sh[16][128];
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int64_t c = (int64_t)blockIdx.x * 128 + tx * 8;
@@ -222,18 +222,13 @@ ds_split_kernel(DsArgs a, const uint32_t *__restrict__ amax, __half *__restrict_
       if (r < a.M && c < a.N) {
         float v[8];
         ds8(a, r, c, v);
-        if (hi) {
-          __half h[8], l[8];
+        __half h[8], l[8];
 #pragma unroll
-          for (int u = 0; u < 8; ++u) half_pair(v[u] * s, h[u], l[u]);
-          *reinterpret_cast<uint4 *>(hi + r * ld + c) = *reinterpret_cast<uint4 *>(h);
-          *reinterpret_cast<uint4 *>(lo + r * ld + c) = *reinterpret_cast<uint4 *>(l);
-        }
+        for (int u = 0; u < 8; ++u) half_pair(v[u] * s, h[u], l[u]);
+        *reinterpret_cast<uint4 *>(hi + r * ld + c) = *reinterpret_cast<uint4 *>(h);
+        *reinterpret_cast<uint4 *>(lo + r * ld + c) = *reinterpret_cast<uint4 *>(l);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          if (ds32 && c + u < a.N) ds32[r * a.N + c + u] = v[u];
-          cs[u] += v[u];
-        }
+        for (int u = 0; u < 8; ++u) cs[u] += v[u];
       }
     }
     if (sums) {
@@ -252,43 +247,30 @@ ds_split_kernel(DsArgs a, const uint32_t *__restrict__ amax, __half *__restrict_
   }
 }
 
-// The tensor-core products take over where a product has enough work to fill a few CTA pairs.
-static bool keep_small(int64_t M, int64_t N, int64_t K) {
-  if (!gemm_f16_available()) return true;
-  return M * K <= ((int64_t)1 << 24) / N;
-}
-
 struct KeepForward { uint32_t *amax; __half *xh, *xl, *wh, *wl; float *partial; int64_t ldx, ldw; };
 static size_t keep_carve_forward(int64_t M, int64_t N, int64_t K, char *base, KeepForward &f) {
   Carver c{base};
   f = KeepForward{};
   f.amax = c.take<uint32_t>(2);
-  if (!keep_small(M, N, K)) {
-    f.ldx = ceil_div(K, 8) * 8; f.ldw = ceil_div(N, 8) * 8;
-    f.xh = c.take<__half>(M * f.ldx); f.xl = c.take<__half>(M * f.ldx);
-    f.wh = c.take<__half>(K * f.ldw); f.wl = c.take<__half>(K * f.ldw);
-    f.partial = reinterpret_cast<float *>(c.take<char>((int64_t)gemm_f16_partial_bytes(M, N, K)));
-  }
+  f.ldx = ceil_div(K, 8) * 8; f.ldw = ceil_div(N, 8) * 8;
+  f.xh = c.take<__half>(M * f.ldx); f.xl = c.take<__half>(M * f.ldx);
+  f.wh = c.take<__half>(K * f.ldw); f.wl = c.take<__half>(K * f.ldw);
+  f.partial = reinterpret_cast<float *>(c.take<char>((int64_t)gemm_f16_partial_bytes(M, N, K)));
   return c.used;
 }
-struct KeepBackward { uint32_t *amax; __half *dh, *dl, *wh, *wl, *x8; float *partial, *sums, *ds32, *x32; int64_t ldd, ldw, ldx; };
+struct KeepBackward { uint32_t *amax; __half *dh, *dl, *wh, *wl, *x8; float *partial, *sums; int64_t ldd, ldw, ldx; };
 static size_t keep_carve_backward(int64_t M, int64_t N, int64_t K, char *base, KeepBackward &f) {
   Carver c{base};
   f = KeepBackward{};
   f.amax = c.take<uint32_t>(2);
   f.sums = c.take<float>(ceil_div(M, 64) * N);
-  if (keep_small(M, N, K)) {
-    f.ds32 = c.take<float>(M * N);
-    f.x32 = c.take<float>(M * K);
-  } else {
-    f.ldd = f.ldw = ceil_div(N, 8) * 8;
-    f.ldx = ceil_div(K, 32) * 32;
-    f.dh = c.take<__half>(M * f.ldd); f.dl = c.take<__half>(M * f.ldd);
-    f.wh = c.take<__half>(K * f.ldw); f.wl = c.take<__half>(K * f.ldw);
-    f.x8 = c.take<__half>(M * f.ldx);
-    const size_t a = gemm_f16_partial_bytes(M, K, N), b = gemm_f16_partial_bytes(K, N, M);
-    f.partial = reinterpret_cast<float *>(c.take<char>((int64_t)(a > b ? a : b)));
-  }
+  f.ldd = f.ldw = ceil_div(N, 8) * 8;
+  f.ldx = ceil_div(K, 32) * 32;
+  f.dh = c.take<__half>(M * f.ldd); f.dl = c.take<__half>(M * f.ldd);
+  f.wh = c.take<__half>(K * f.ldw); f.wl = c.take<__half>(K * f.ldw);
+  f.x8 = c.take<__half>(M * f.ldx);
+  const size_t a = gemm_f16_partial_bytes(M, K, N), b = gemm_f16_partial_bytes(K, N, M);
+  f.partial = reinterpret_cast<float *>(c.take<char>((int64_t)(a > b ? a : b)));
   return c.used;
 }
 
@@ -365,16 +347,15 @@ int endia_b200_linear_keep_fwd(const float *x, int64_t ldx, const float *W, int6
   EB_REQUIRE(x && ldx >= K && (N == 0 || (W && out && ldw >= N)), ENDIA_B200_EINVAL, "linear_keep: NULL pointer or leading dimension too small");
   if (kept_x && (st = run_keep8(x, ldx, M, K, keep_sign, kept_x, s))) return st;
   if (N == 0) return ENDIA_B200_OK;
-  if (keep_small(M, N, K)) return gemm_fp32(0, 0, M, N, K, x, ldx, W, ldw, out, N, bias, act, 0.f, s);
   KeepForward f;
   keep_carve_forward(M, N, K, static_cast<char *>(scratch), f);
   EB_CUDA(cudaMemsetAsync(f.amax, 0, 2 * sizeof(uint32_t), s));
   // the 8-bit form has found the largest |x| already
-  const uint32_t *amax_x = kept_x ? static_cast<const uint32_t *>(kept_x) : f.amax;
-  if (!kept_x && (st = launch_amax(x, M, K, ldx, nullptr, f.amax, s))) return st;
-  if ((st = launch_amax(W, K, N, ldw, nullptr, f.amax + 1, s))) return st;
-  if ((st = launch_half_split(x, M, K, ldx, nullptr, amax_x, f.xh, f.xl, f.ldx, s))) return st;
-  if ((st = launch_half_split(W, K, N, ldw, nullptr, f.amax + 1, f.wh, f.wl, f.ldw, s))) return st;
+  uint32_t *amax_x = kept_x ? static_cast<uint32_t *>(kept_x) : f.amax;
+  HalfJob jw{W, K, N, ldw, nullptr, f.amax + 1, f.wh, f.wl, f.ldw};
+  HalfJob jx{x, M, K, ldx, nullptr, amax_x, f.xh, f.xl, f.ldx};
+  if ((st = launch_amax(jw, kept_x ? nullptr : &jx, s))) return st;
+  if ((st = launch_half_split(jw, &jx, s))) return st;
   F16Gemm g;
   g.M = M; g.N = N; g.K = K;
   g.a = HalfPair{f.xh, f.xl, f.ldx, amax_x};
@@ -402,30 +383,18 @@ int endia_b200_linear_keep_bwd(const void *kept_x, const float *W, int64_t ldw, 
              "linear_keep: NULL pointer or leading dimension too small");
   KeepBackward f;
   keep_carve_backward(M, N, K, static_cast<char *>(scratch), f);
-  const bool small = keep_small(M, N, K);
   DsArgs a{};
   a.g = grad; a.out = act && out ? out : nullptr; a.act = act; a.M = M; a.N = N;
   if (act && !out) a.kept = kept_view(const_cast<void *>(kept_out), M, N);
   a.vec = N % 4 == 0 && (reinterpret_cast<uintptr_t>(grad) & 15) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
   const dim3 grid((unsigned)ceil_div(N, 128), (unsigned)(ceil_div(M, 64) < 32768 ? ceil_div(M, 64) : 32768));
-  if (!small) {
-    EB_CUDA(cudaMemsetAsync(f.amax, 0, 2 * sizeof(uint32_t), s));
-    ds_amax_kernel<<<grid_for(M * ceil_div(N, 8), 256, 8), 256, 0, s>>>(a, f.amax);
-    EB_LAUNCH_CHECK();
-  }
-  ds_split_kernel<<<grid, 256, 0, s>>>(a, f.amax, f.dh, f.dl, f.ldd, f.ds32, db ? f.sums : nullptr);
+  EB_CUDA(cudaMemsetAsync(f.amax, 0, 2 * sizeof(uint32_t), s));
+  ds_amax_kernel<<<grid_for(M * ceil_div(N, 8), 256, 8), 256, 0, s>>>(a, f.amax);
+  EB_LAUNCH_CHECK();
+  ds_split_kernel<<<grid, 256, 0, s>>>(a, f.amax, f.dh, f.dl, f.ldd, db ? f.sums : nullptr);
   EB_LAUNCH_CHECK();
   if (db && (st = launch_column_sums(f.sums, (int)ceil_div(M, 64), N, nullptr, db, s))) return st;
   const Kept kx = kept_view(const_cast<void *>(kept_x), M, K);
-  if (small) {
-    if (dx && (st = gemm_fp32(0, 1, M, K, N, f.ds32, N, W, ldw, dx, K, nullptr, 0, 0.f, s))) return st;
-    if (dw) {
-      kept_read_kernel<<<grid_for(M * (kx.ldq / 8), 256, 8), 256, 0, s>>>(kx, M, K, f.x32);
-      EB_LAUNCH_CHECK();
-      return gemm_fp32(1, 0, K, N, M, f.x32, K, f.ds32, N, dw, N, nullptr, 0, 0.f, s);
-    }
-    return ENDIA_B200_OK;
-  }
   const HalfPair d{f.dh, f.dl, f.ldd, f.amax};
   if (dw) {
     kept_half_kernel<<<grid_for(M * (kx.ldq / 16), 256, 8), 256, 0, s>>>(kx, M, f.x8);
@@ -438,8 +407,9 @@ int endia_b200_linear_keep_bwd(const void *kept_x, const float *W, int64_t ldw, 
     if ((st = launch_gemm_f16(g, true, true, F16_STORE, s))) return st;
   }
   if (dx) {
-    if ((st = launch_amax(W, K, N, ldw, nullptr, f.amax + 1, s))) return st;
-    if ((st = launch_half_split(W, K, N, ldw, nullptr, f.amax + 1, f.wh, f.wl, f.ldw, s))) return st;
+    const HalfJob jw{W, K, N, ldw, nullptr, f.amax + 1, f.wh, f.wl, f.ldw};
+    if ((st = launch_amax(jw, nullptr, s))) return st;
+    if ((st = launch_half_split(jw, nullptr, s))) return st;
     F16Gemm g;
     g.M = M; g.N = K; g.K = N;
     g.a = d;

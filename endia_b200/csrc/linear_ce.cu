@@ -7,7 +7,7 @@
 // vocabulary the logits are formed again, d leaves the epilogue as an fp16 pair (|d| <= 1, a fixed
 // scale), and feeds the two gradient products of the piece. 8 M K V multiply-adds instead of the 6
 // that kept logits would take, at 4 (M + K) bytes of work space per column of a piece.
-// Large problems run on the fp16-pair tensor-core kernel (gemm_f16.cuh), small ones on the fp32 kernels.
+// The products run on the fp16-pair tensor-core kernel (gemm_f16.cuh), but the forward one of up to 16 rows.
 // The reference's one loss is mse (endia/functional/loss_ops/mse_op.mojo:18-20); this is the
 // classification loss beside it.
 #include "gemm_f16.cuh"
@@ -18,8 +18,8 @@ using namespace eb;
 
 namespace eb {
 
-// state: [0] rows that count, [1] and [2] the scales' maxima of x and W (bits), [4 ...) lse per row, then
-// lse log2 e per row. Inside, logits are in units of log2 e: exponentials are powers of two.
+// state: [0] rows that count, [1] and [2] the scales' maxima of x and W (bits), [3] CTAs of ce_rows_kernel
+// that are done, [4 ...) lse per row, then lse log2 e per row. Inside, logits are in units of log2 e: exponentials are powers of two.
 constexpr double CE_LOG2E = 1.4426950408889634, CE_LN2 = 0.6931471805599453;
 constexpr int CE_STATE_HEAD = 4;
 // Work space for one piece of the vocabulary (the d pair and W's pair, 4 bytes each per element).
@@ -31,12 +31,20 @@ constexpr int CE_MAX_CLASSES = 1 << 24;    // class numbers are float32 values
 __device__ __forceinline__ bool ce_invalid(float t, int V) { return !(t < (float)V) || t != floorf(t); }
 
 // ------------------------------------------------------------------------------------- forward, second part
-// Rows of a CTA: 32; its 16 warps take the parts of a row's (max, sum) in turn, lanes along the rows.
+// Joins a row's (max, sum) parts; rows of a CTA: 32, its 16 warps take the parts in turn, lanes along the
+// rows. The CTA that finishes last adds up the rows' losses and the rows that count, in a fixed order.
+__device__ __forceinline__ void ce_join(float &mx, float &sum, float2 v) {
+  const float nm = fmaxf(mx, v.x);
+  if (nm > -INFINITY) sum = sum * exp2f(mx - nm) + v.y * exp2f(v.x - nm);
+  else sum += v.y;      // (0, or NaN)
+  mx = nm;
+}
 __global__ void __launch_bounds__(512)
 ce_rows_kernel(const float2 *__restrict__ stats, int parts, const float *__restrict__ target,
-               const float *__restrict__ target_logit, int M, int V, float *__restrict__ lse, float *__restrict__ lse2,
-               float *__restrict__ row_loss) {
+               const float *__restrict__ target_logit, int M, int V, float *__restrict__ state, float *row_loss,
+               int mean, float *__restrict__ loss) {
   __shared__ float2 part[16][32];
+  __shared__ int last;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int m = (int)blockIdx.x * 32 + lane;
   float mx = -INFINITY, sum = 0.f;
@@ -46,63 +54,43 @@ ce_rows_kernel(const float2 *__restrict__ stats, int parts, const float *__restr
 #pragma unroll
       for (int u = 0; u < 8; ++u) v[u] = p0 + 16 * u < parts ? __ldcs(stats + (int64_t)(p0 + 16 * u) * M + m) : make_float2(-INFINITY, 0.f);
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float nm = fmaxf(mx, v[u].x);
-        if (nm > -INFINITY) sum = sum * exp2f(mx - nm) + v[u].y * exp2f(v[u].x - nm);
-        else sum += v[u].y;      // (0, or NaN)
-        mx = nm;
-      }
+      for (int u = 0; u < 8; ++u) ce_join(mx, sum, v[u]);
     }
   }
   part[w][lane] = make_float2(mx, sum);
   __syncthreads();
   if (w == 0 && m < M) {
-    for (int i = 1; i < 16; ++i) {
-      const float2 v = part[i][lane];
-      const float nm = fmaxf(mx, v.x);
-      if (nm > -INFINITY) sum = sum * exp2f(mx - nm) + v.y * exp2f(v.x - nm);
-      else sum += v.y;
-      mx = nm;
-    }
+    for (int i = 1; i < 16; ++i) ce_join(mx, sum, part[i][lane]);
     const float t = __ldg(target + m);
     const double l2 = (double)mx + (double)log2f(sum);
-    lse[m] = (float)(l2 * CE_LN2);
-    lse2[m] = (float)l2;
+    state[CE_STATE_HEAD + m] = (float)(l2 * CE_LN2);
+    state[CE_STATE_HEAD + M + m] = (float)l2;
     row_loss[m] = t < 0.f ? 0.f : (ce_invalid(t, V) ? NAN : (float)((l2 - (double)target_logit[m]) * CE_LN2));
+    __threadfence();
   }
-}
-
-// loss[0] = sum of the rows' losses (over the number of rows that count, when mean), in a fixed order.
-__global__ void __launch_bounds__(1024)
-ce_loss_kernel(const float *__restrict__ row_loss, const float *__restrict__ target, int M, int mean,
-               float *__restrict__ loss, float *__restrict__ count_out) {
-  __shared__ float ps[32];
-  __shared__ int pc[32];
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(reinterpret_cast<unsigned int *>(state) + 3, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
   float s = 0.f;
   int c = 0;
-  for (int m = threadIdx.x; m < M; m += 1024) {
-    s += row_loss[m];
-    c += !(target[m] < 0.f);
+  for (int i = threadIdx.x; i < M; i += 512) {
+    s += __ldcg(row_loss + i);
+    c += !(__ldg(target + i) < 0.f);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     s += __shfl_xor_sync(0xffffffffu, s, o);
     c += __shfl_xor_sync(0xffffffffu, c, o);
   }
-  if ((threadIdx.x & 31) == 0) { ps[threadIdx.x >> 5] = s; pc[threadIdx.x >> 5] = c; }
+  if (lane == 0) part[0][w] = make_float2(s, __int_as_float(c));
   __syncthreads();
-  if (threadIdx.x < 32) {
-    s = ps[threadIdx.x];
-    c = pc[threadIdx.x];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      s += __shfl_xor_sync(0xffffffffu, s, o);
-      c += __shfl_xor_sync(0xffffffffu, c, o);
-    }
-    if (threadIdx.x == 0) {
-      if (loss) loss[0] = c == 0 ? 0.f : (mean ? s / (float)c : s);
-      count_out[0] = (float)c;
-    }
+  if (threadIdx.x == 0) {
+    s = 0.f;
+    c = 0;
+    for (int i = 0; i < 16; ++i) { s += part[0][i].x; c += __float_as_int(part[0][i].y); }
+    if (loss) loss[0] = c == 0 ? 0.f : (mean ? s / (float)c : s);
+    state[0] = (float)c;
   }
 }
 
@@ -140,84 +128,111 @@ ce_coef_kernel(const float *__restrict__ g, int per_row, int mean, const float *
   }
 }
 
-// ------------------------------------------------------------------------------------ small problems, fp32
-// (max, sum) and the target's logit of one row of a piece; one CTA per row.
+// ------------------------------------------------------------------------------------ few rows, fp32
+// The statistics of up to 16 rows in one pass over W, which is all that such a call has to read: a CTA takes 128
+// columns, its eight warps take the features in turn (x as [feature][row] in shared memory, four columns
+// and ROWS x 4 sums a lane), and eight loads of 128 bits a lane are in flight. The warps' sums are added in
+// order, then a warp per row (two rows) reduces 128 logits as the tensor-core epilogue does.
+constexpr int CE_FEW = 16, CE_FEW_K = 512;
+template <int ROWS, bool VEC>
 __global__ void __launch_bounds__(256)
-ce_piece_stats_kernel(const float *__restrict__ l, int64_t ld, int N, int n_base, const float *__restrict__ target, int M,
-                      float2 *__restrict__ stats, float *__restrict__ target_logit) {
-  __shared__ float sh[8];
+ce_few_rows_kernel(const float *__restrict__ x, int64_t ldx, const float *__restrict__ W, int64_t ldw, const float *__restrict__ bias,
+                   const float *__restrict__ target, int M, int K, int V, float2 *__restrict__ stats, float *__restrict__ target_logit) {
+  __shared__ __align__(16) float xs[CE_FEW_K][ROWS];
+  __shared__ float red[ROWS][128];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  for (int m = (int)blockIdx.x; m < M; m += (int)gridDim.x) {
-    const float *row = l + (int64_t)m * ld;
-    float mx = -INFINITY;
-    for (int n = threadIdx.x; n < N; n += 256) mx = fmaxf(mx, row[n] * (float)CE_LOG2E);
+  const int n0 = (int)blockIdx.x * 128;
+  // this lane's four columns: consecutive, or 32 apart where rows of W are not 16-byte aligned
+  int col[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) col[j] = n0 + (VEC ? 4 * lane + j : lane + 32 * j);
+  float acc[ROWS][4];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[r][j] = 0.f;
+  const bool inside = n0 + 128 <= V;
+  for (int k0 = 0; k0 < K; k0 += CE_FEW_K) {
+    const int kn = K - k0 < CE_FEW_K ? K - k0 : CE_FEW_K;
+    __syncthreads();
+    for (int i = threadIdx.x; i < ROWS * kn; i += 256) {
+      const int r = i / kn, k = i - r * kn;
+      xs[k][r] = r < M ? __ldg(x + (int64_t)r * ldx + k0 + k) : 0.f;
+    }
+    __syncthreads();
+    for (int kb = w; kb < kn; kb += 64) {
+      float v[8][4];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int k = kb + 8 * u;
+        const float *row = W + (int64_t)(k0 + k) * ldw;
+        if (VEC && inside) {
+          const float4 q = k < kn ? __ldcs(reinterpret_cast<const float4 *>(row + col[0])) : make_float4(0.f, 0.f, 0.f, 0.f);
+          v[u][0] = q.x; v[u][1] = q.y; v[u][2] = q.z; v[u][3] = q.w;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[u][j] = k < kn && col[j] < V ? __ldcs(row + col[j]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int k = kb + 8 * u;
+        if (k < kn) {
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r) {
+            const float xv = xs[k][r];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[r][j] = fmaf(xv, v[u][j], acc[r][j]);
+          }
+        }
+      }
+    }
+  }
+  for (int src = 0; src < 8; ++src) {
+    if (w == src) {
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) red[r][col[j] - n0] = src ? red[r][col[j] - n0] + acc[r][j] : acc[r][j];
+    }
+    __syncthreads();
+  }
+  for (int m = w; m < M; m += 8) {
+    const float tg = __ldg(target + m);
+    float l[4], mx = -INFINITY, s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = n0 + lane + 32 * j;
+      l[j] = n < V ? (red[m][lane + 32 * j] + (bias ? __ldg(bias + n) : 0.f)) * (float)CE_LOG2E : -INFINITY;
+      mx = fmaxf(mx, l[j]);
+      if (n < V && tg == (float)n) target_logit[m] = l[j];
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    __syncthreads();
-    if (lane == 0) sh[w] = mx;
-    __syncthreads();
+    const float base = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) mx = fmaxf(mx, sh[i]);
-    float s = 0.f;
-    for (int n = threadIdx.x; n < N; n += 256) {
-      const float v = row[n] * (float)CE_LOG2E;
-      s += v == -INFINITY ? 0.f : exp2f(v - mx);
-    }
+    for (int j = 0; j < 4; ++j) s += exp2f(l[j] - base);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    __syncthreads();
-    if (lane == 0) sh[w] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      s = 0.f;
-      for (int i = 0; i < 8; ++i) s += sh[i];
-      stats[m] = make_float2(mx, s);
-      const float t = target[m];
-      if (t >= (float)n_base && t < (float)(n_base + N)) target_logit[m] = row[(int)t - n_base] * (float)CE_LOG2E;
-    }
+    if (lane == 0) stats[(int64_t)blockIdx.x * M + m] = make_float2(mx, s);
   }
 }
 
-// logits -> d, in place (with the whole gradient factor; fp32 needs no scale).
-__global__ void __launch_bounds__(256)
-ce_piece_d_kernel(float *__restrict__ l, int64_t ld, int N, int n_base, const float *__restrict__ target, int M,
-                  const float *__restrict__ lse, const float *__restrict__ coef, const float *__restrict__ alpha) {
-  const int64_t total = (int64_t)M * N, step = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
-    const int m = (int)(i / N), n = (int)(i - (int64_t)m * N);
-    const float c = coef[m];
-    const float e = exp2f(l[(int64_t)m * ld + n] * (float)CE_LOG2E - lse[m]) - (target[m] == (float)(n_base + n) ? 1.f : 0.f);
-    l[(int64_t)m * ld + n] = c == 0.f ? 0.f : e * (c * __ldg(alpha));
-  }
+template <int ROWS>
+static int launch_few_rows(const float *x, int64_t ldx, const float *W, int64_t ldw, const float *bias, const float *target, int M,
+                           int K, int V, float2 *stats, float *target_logit, cudaStream_t s) {
+  const unsigned grid = (unsigned)ceil_div(V, 128);
+  if (ldw % 4 == 0 && (reinterpret_cast<uintptr_t>(W) & 15) == 0)
+    ce_few_rows_kernel<ROWS, true><<<grid, 256, 0, s>>>(x, ldx, W, ldw, bias, target, M, K, V, stats, target_logit);
+  else
+    ce_few_rows_kernel<ROWS, false><<<grid, 256, 0, s>>>(x, ldx, W, ldw, bias, target, M, K, V, stats, target_logit);
+  EB_LAUNCH_CHECK();
+  return ENDIA_B200_OK;
 }
 
-// x with the rows that are left out as zeros.
-__global__ void __launch_bounds__(256)
-ce_rows_copy_kernel(const float *__restrict__ x, int64_t ld, const float *__restrict__ target, int M, int K, float *__restrict__ out) {
-  const int64_t total = (int64_t)M * K, step = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
-    const int64_t m = i / K;
-    out[i] = target[m] < 0.f ? 0.f : x[m * ld + (i - m * K)];
-  }
-}
-
-__global__ void __launch_bounds__(256)
-ce_colsum_kernel(const float *__restrict__ d, int64_t ld, int M, int N, float *__restrict__ db) {
-  const int n = (int)(blockIdx.x * blockDim.x + threadIdx.x);
-  if (n >= N) return;
-  float s = 0.f;
-#pragma unroll 8
-  for (int m = 0; m < M; ++m) s += d[(int64_t)m * ld + n];
-  db[n] = s;
-}
-
-// The fp32 kernels take what is too small to fill the tensor-core kernel: few classes and few
-// multiply-adds, or, without gradients, at most 8 rows (one pass over W).
-static bool ce_small(int64_t M, int64_t K, int64_t V, bool backward) {
-  if (!gemm_f16_available()) return true;
-  if (!backward && M <= 8) return true;
-  return V <= 4096 && M * K <= ((int64_t)1 << 24) / V;
-}
+// Up to 16 rows the forward pass reads W once and is done (4 bytes per weight; making pairs first costs 16);
+// its multiply-adds stay below the time of that read on the fp32 pipes.
+static bool ce_few_rows(int64_t M) { return M <= CE_FEW; }
 
 // Columns per piece: equal pieces (multiples of 256) whose work space stays near CE_PIECE_BYTES.
 static int64_t ce_piece(int64_t bytes_per_column, int64_t V) {
@@ -227,16 +242,14 @@ static int64_t ce_piece(int64_t bytes_per_column, int64_t V) {
   return ceil_div(ceil_div(V, pieces), 256) * 256;
 }
 
-struct CeForward { float2 *stats; float *tl, *rows, *logits, *unused; __half *xh, *xl, *wh, *wl; int64_t piece, parts, ldx; };
+struct CeForward { float2 *stats; float *tl, *rows; __half *xh, *xl, *wh, *wl; int64_t piece, parts, ldx; };
 static size_t ce_carve_forward(int64_t M, int64_t K, int64_t V, char *base, CeForward &f) {
   Carver c{base};
   f = CeForward{};
   f.tl = c.take<float>(M);
   f.rows = c.take<float>(M);
-  if (ce_small(M, K, V, false)) {
-    f.piece = ce_piece(4 * M, V);
-    f.parts = ceil_div(V, f.piece);
-    f.logits = c.take<float>(M * f.piece);
+  if (ce_few_rows(M)) {
+    f.parts = ceil_div(V, 128);
   } else {
     f.piece = ce_piece(4 * K, V);
     f.parts = 2 * ceil_div(V, 256);
@@ -248,30 +261,24 @@ static size_t ce_carve_forward(int64_t M, int64_t K, int64_t V, char *base, CeFo
   return c.used;
 }
 
-struct CeBackward { float *coef, *alpha, *partial, *part_sums, *d, *x0; uint32_t *amax; __half *xh, *xl, *wh, *wl, *dh, *dl; int64_t piece, ldx; };
+struct CeBackward { float *coef, *alpha, *partial, *part_sums; uint32_t *amax; __half *xh, *xl, *wh, *wl, *dh, *dl; int64_t piece, ldx; };
 static size_t ce_carve_backward(int64_t M, int64_t K, int64_t V, char *base, CeBackward &f) {
   Carver c{base};
   f = CeBackward{};
   f.coef = c.take<float>(M);
   f.alpha = c.take<float>(2);
   f.amax = c.take<uint32_t>(2);
-  if (ce_small(M, K, V, true)) {
-    f.piece = ce_piece(4 * M, V);
-    f.d = c.take<float>(M * f.piece);
-    f.x0 = c.take<float>(M * K);
-  } else {
-    f.piece = ce_piece(4 * (M + K), V);
-    f.ldx = ceil_div(K, 8) * 8;
-    f.xh = c.take<__half>(M * f.ldx); f.xl = c.take<__half>(M * f.ldx);
-    f.wh = c.take<__half>(K * f.piece); f.wl = c.take<__half>(K * f.piece);
-    f.dh = c.take<__half>(M * f.piece); f.dl = c.take<__half>(M * f.piece);
-    f.part_sums = c.take<float>(ceil_div(M, 32) * f.piece);
-    size_t a = gemm_f16_partial_bytes(M, K, f.piece), b = gemm_f16_partial_bytes(K, f.piece, M);
-    const int64_t last = V - (ceil_div(V, f.piece) - 1) * f.piece;      // the last piece may be cut otherwise
-    const size_t a2 = gemm_f16_partial_bytes(M, K, last), b2 = gemm_f16_partial_bytes(K, last, M);
-    a = a > a2 ? a : a2; b = b > b2 ? b : b2;
-    f.partial = reinterpret_cast<float *>(c.take<char>((int64_t)(a > b ? a : b)));
-  }
+  f.piece = ce_piece(4 * (M + K), V);
+  f.ldx = ceil_div(K, 8) * 8;
+  f.xh = c.take<__half>(M * f.ldx); f.xl = c.take<__half>(M * f.ldx);
+  f.wh = c.take<__half>(K * f.piece); f.wl = c.take<__half>(K * f.piece);
+  f.dh = c.take<__half>(M * f.piece); f.dl = c.take<__half>(M * f.piece);
+  f.part_sums = c.take<float>(ceil_div(M, 32) * f.piece);
+  size_t a = gemm_f16_partial_bytes(M, K, f.piece), b = gemm_f16_partial_bytes(K, f.piece, M);
+  const int64_t last = V - (ceil_div(V, f.piece) - 1) * f.piece;      // the last piece may be cut otherwise
+  const size_t a2 = gemm_f16_partial_bytes(M, K, last), b2 = gemm_f16_partial_bytes(K, last, M);
+  a = a > a2 ? a : a2; b = b > b2 ? b : b2;
+  f.partial = reinterpret_cast<float *>(c.take<char>((int64_t)(a > b ? a : b)));
   return c.used;
 }
 
@@ -320,21 +327,18 @@ int endia_b200_linear_ce_fwd(const float *x, int64_t ldx, const float *W, int64_
   ce_carve_forward(M, K, V, static_cast<char *>(scratch), f);
   float *rows = reduction == ENDIA_B200_LOSS_NONE ? loss : f.rows;
   uint32_t *amax = reinterpret_cast<uint32_t *>(state) + 1;
-  if (ce_small(M, K, V, false)) {
-    for (int64_t v0 = 0, i = 0; v0 < V; v0 += f.piece, ++i) {
-      const int64_t n = V - v0 < f.piece ? V - v0 : f.piece;
-      if ((st = gemm_fp32(0, 0, M, n, K, x, ldx, W + v0, ldw, f.logits, f.piece, bias ? bias + v0 : nullptr, 0, 0.f, s))) return st;
-      ce_piece_stats_kernel<<<(unsigned)(M < 4096 ? M : 4096), 256, 0, s>>>(f.logits, f.piece, (int)n, (int)v0, target, (int)M,
-                                                                           f.stats + i * M, f.tl);
-      EB_LAUNCH_CHECK();
-    }
+  if (ce_few_rows(M)) {
+    const auto few = M <= 1 ? launch_few_rows<1> : M <= 2 ? launch_few_rows<2> : M <= 4 ? launch_few_rows<4>
+                     : M <= 8 ? launch_few_rows<8> : launch_few_rows<CE_FEW>;
+    if ((st = few(x, ldx, W, ldw, bias, target, (int)M, (int)K, (int)V, f.stats, f.tl, s))) return st;
   } else {
-    if ((st = launch_amax(x, M, K, ldx, target, amax, s))) return st;
-    if ((st = launch_amax(W, K, V, ldw, nullptr, amax + 1, s))) return st;
-    if ((st = launch_half_split(x, M, K, ldx, target, amax, f.xh, f.xl, f.ldx, s))) return st;
+    const HalfJob jx{x, M, K, ldx, target, amax, f.xh, f.xl, f.ldx};
+    HalfJob jw{W, K, V, ldw, nullptr, amax + 1, f.wh, f.wl, f.piece};
+    if ((st = launch_amax(jw, &jx, s))) return st;
     for (int64_t v0 = 0; v0 < V; v0 += f.piece) {
       const int64_t n = V - v0 < f.piece ? V - v0 : f.piece;
-      if ((st = launch_half_split(W + v0, K, n, ldw, nullptr, amax + 1, f.wh, f.wl, f.piece, s))) return st;
+      jw.x = W + v0; jw.cols = n;
+      if ((st = launch_half_split(jw, v0 ? nullptr : &jx, s))) return st;
       F16Gemm g;
       g.M = M; g.N = n; g.K = K;
       g.a = HalfPair{f.xh, f.xl, f.ldx, amax};
@@ -344,11 +348,9 @@ int endia_b200_linear_ce_fwd(const float *x, int64_t ldx, const float *W, int64_
       if ((st = launch_gemm_f16(g, false, true, F16_STATS, s))) return st;
     }
   }
-  ce_rows_kernel<<<(unsigned)ceil_div(M, 32), 512, 0, s>>>(f.stats, (int)f.parts, target, f.tl, (int)M, (int)V,
-                                                           state + CE_STATE_HEAD, state + CE_STATE_HEAD + M, rows);
-  EB_LAUNCH_CHECK();
-  ce_loss_kernel<<<1, 1024, 0, s>>>(rows, target, (int)M, reduction == ENDIA_B200_LOSS_MEAN,
-                                    reduction == ENDIA_B200_LOSS_NONE ? nullptr : loss, state);
+  ce_rows_kernel<<<(unsigned)ceil_div(M, 32), 512, 0, s>>>(f.stats, (int)f.parts, target, f.tl, (int)M, (int)V, state, rows,
+                                                           reduction == ENDIA_B200_LOSS_MEAN,
+                                                           reduction == ENDIA_B200_LOSS_NONE ? nullptr : loss);
   EB_LAUNCH_CHECK();
   return ENDIA_B200_OK;
 }
@@ -370,40 +372,21 @@ int endia_b200_linear_ce_bwd(const float *x, int64_t ldx, const float *W, int64_
   CeBackward f;
   ce_carve_backward(M, K, V, static_cast<char *>(scratch), f);
   const float *lse = state + CE_STATE_HEAD + M;      // (in units of log2 e)
-  const uint32_t *amax = reinterpret_cast<const uint32_t *>(state) + 1;
-  const bool small = ce_small(M, K, V, true);
+  uint32_t *amax = const_cast<uint32_t *>(reinterpret_cast<const uint32_t *>(state)) + 1;      // (read only)
   ce_coef_kernel<<<1, 1024, 0, s>>>(grad, reduction == ENDIA_B200_LOSS_NONE, reduction == ENDIA_B200_LOSS_MEAN, state, target,
                                     (int)M, (int)V, f.coef, f.alpha);
   EB_LAUNCH_CHECK();
-  if (small) {
-    if (dw) {
-      ce_rows_copy_kernel<<<grid_for(M * K, 256), 256, 0, s>>>(x, ldx, target, (int)M, (int)K, f.x0);
-      EB_LAUNCH_CHECK();
-    }
-    for (int64_t v0 = 0; v0 < V; v0 += f.piece) {
-      const int64_t n = V - v0 < f.piece ? V - v0 : f.piece;
-      if ((st = gemm_fp32(0, 0, M, n, K, x, ldx, W + v0, ldw, f.d, f.piece, bias ? bias + v0 : nullptr, 0, 0.f, s))) return st;
-      ce_piece_d_kernel<<<grid_for(M * n, 256), 256, 0, s>>>(f.d, f.piece, (int)n, (int)v0, target, (int)M, lse, f.coef, f.alpha);
-      EB_LAUNCH_CHECK();
-      if (dx && (st = gemm_fp32(0, 1, M, K, n, f.d, f.piece, W + v0, ldw, dx, K, nullptr, 0, v0 ? 1.f : 0.f, s))) return st;
-      if (dw && (st = gemm_fp32(1, 0, K, n, M, f.x0, K, f.d, f.piece, dw + v0, V, nullptr, 0, 0.f, s))) return st;
-      if (db) {
-        ce_colsum_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, s>>>(f.d, f.piece, (int)M, (int)n, db + v0);
-        EB_LAUNCH_CHECK();
-      }
-    }
-    return ENDIA_B200_OK;
-  }
-  if (ce_small(M, K, V, false)) {      // the forward pass ran in fp32 and left no scales
+  HalfJob jx{x, M, K, ldx, target, amax, f.xh, f.xl, f.ldx}, jw{W, K, V, ldw, nullptr, amax + 1, f.wh, f.wl, f.piece};
+  if (ce_few_rows(M)) {      // the forward pass ran in fp32 and left no scales
+    jx.amax = amax = f.amax;
+    jw.amax = amax + 1;
     EB_CUDA(cudaMemsetAsync(f.amax, 0, 2 * sizeof(uint32_t), s));
-    if ((st = launch_amax(x, M, K, ldx, target, f.amax, s))) return st;
-    if ((st = launch_amax(W, K, V, ldw, nullptr, f.amax + 1, s))) return st;
-    amax = f.amax;
+    if ((st = launch_amax(jw, &jx, s))) return st;
   }
-  if ((st = launch_half_split(x, M, K, ldx, target, amax, f.xh, f.xl, f.ldx, s))) return st;
   for (int64_t v0 = 0; v0 < V; v0 += f.piece) {
     const int64_t n = V - v0 < f.piece ? V - v0 : f.piece;
-    if ((st = launch_half_split(W + v0, K, n, ldw, nullptr, amax + 1, f.wh, f.wl, f.piece, s))) return st;
+    jw.x = W + v0; jw.cols = n;
+    if ((st = launch_half_split(jw, v0 ? nullptr : &jx, s))) return st;
     F16Gemm g;
     g.M = M; g.N = n; g.K = K;
     g.a = HalfPair{f.xh, f.xl, f.ldx, amax};
