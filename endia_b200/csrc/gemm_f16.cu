@@ -41,6 +41,7 @@ struct F16Params {
   int pairs_m, tiles_n, group_m, ksplit, nkb;   // nkb: stages of 64 of K in all
   const uint32_t *amax_a, *amax_b;
   const float *alpha_dev;
+  int alpha_exp;
   const float *bias;
   float *C;
   int64_t ldc;
@@ -239,8 +240,8 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
     const uint32_t ebuf = epi_base + (uint32_t)(warp - 4) * 4096u;
     const uint32_t row_addr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * 128);
     const uint32_t empty_leader[2] = {map_to_cta(acc_empty(0), 0), map_to_cta(acc_empty(1), 0)};
-    const float f0 = half_unscale(p.amax_a);
-    const float f1 = half_unscale(p.amax_b) * (p.alpha_dev ? __ldg(p.alpha_dev) : 1.f);
+    float f0, f1;
+    unscale_factors(p.amax_a, p.amax_b, p.alpha_dev, p.alpha_exp, f0, f1);
     // For logits one factor: where 2^-(e_a + e_b) leaves the range of fp32 it is held at the range's end (the
     // logits are then below 2^-80, or beyond what their fp32 sum could hold)
     const int e_ce = -((p.amax_a ? half_scale_exponent(*p.amax_a) : 0) + (p.amax_b ? half_scale_exponent(*p.amax_b) : 0));
@@ -452,8 +453,8 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
 // thread (the rows of the work space are 16-byte aligned).
 __global__ void __launch_bounds__(256)
 gemm_f16_finish_kernel(const F16Params p, const float *__restrict__ partial, int64_t ld_partial, int64_t slice, int parts) {
-  const float f0 = half_unscale(p.amax_a);
-  const float f1 = half_unscale(p.amax_b) * (p.alpha_dev ? __ldg(p.alpha_dev) : 1.f);
+  float f0, f1;
+  unscale_factors(p.amax_a, p.amax_b, p.alpha_dev, p.alpha_exp, f0, f1);
   const uint32_t per_row = (uint32_t)((p.N + 3) / 4);
   const int64_t total = (int64_t)p.M * per_row, step = (int64_t)gridDim.x * blockDim.x;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
@@ -488,10 +489,11 @@ gemm_f16_finish_kernel(const F16Params p, const float *__restrict__ partial, int
   }
 }
 
-// out[n] = alpha * sum over the parts [parts][N], in a fixed order: 32 columns per CTA, its eight warps take
+// out[n] = alpha * scale * sum over the parts [parts][N], in a fixed order: 32 columns per CTA, its eight warps take
 // the parts in turn with eight loads in flight.
 __global__ void __launch_bounds__(256)
-column_sums_kernel(const float *__restrict__ part, int parts, int64_t N, const float *__restrict__ alpha, float *__restrict__ out) {
+column_sums_kernel(const float *__restrict__ part, int parts, int64_t N, float scale, const float *__restrict__ alpha,
+                   float *__restrict__ out) {
   __shared__ float sh[8][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t n = (int64_t)blockIdx.x * 32 + lane;
@@ -509,12 +511,13 @@ column_sums_kernel(const float *__restrict__ part, int parts, int64_t N, const f
   __syncthreads();
   if (w == 0 && n < N) {
     for (int i = 1; i < 8; ++i) s += sh[i][lane];
+    s *= scale;
     out[n] = alpha ? s * __ldg(alpha) : s;
   }
 }
 
-int launch_column_sums(const float *part, int parts, int64_t N, const float *alpha, float *out, cudaStream_t s) {
-  column_sums_kernel<<<(unsigned)ceil_div(N, 32), 256, 0, s>>>(part, parts, N, alpha, out);
+int launch_column_sums(const float *part, int parts, int64_t N, float scale, const float *alpha, float *out, cudaStream_t s) {
+  column_sums_kernel<<<(unsigned)ceil_div(N, 32), 256, 0, s>>>(part, parts, N, scale, alpha, out);
   EB_LAUNCH_CHECK();
   return ENDIA_B200_OK;
 }
@@ -712,7 +715,7 @@ int launch_gemm_f16(const F16Gemm &g, bool a_mn, bool b_mn, int epilogue, cudaSt
   p.group_m = 8;
   p.nkb = (int)ceil_div(g.K, F16_BK);
   p.ksplit = 1;
-  p.amax_a = g.a.amax; p.amax_b = g.b.amax; p.alpha_dev = g.alpha_dev; p.bias = g.bias;
+  p.amax_a = g.a.amax; p.amax_b = g.b.amax; p.alpha_dev = g.alpha_dev; p.alpha_exp = g.alpha_exp; p.bias = g.bias;
   p.C = g.C; p.ldc = g.ldc; p.act = g.act; p.accumulate = g.accumulate ? 1 : 0;
   p.target = g.target; p.n_base = g.n_base; p.stats = g.stats; p.target_logit = g.target_logit;
   p.lse = g.lse; p.coef = g.coef; p.colsum_part = g.colsum_part;

@@ -23,12 +23,14 @@ enum F16Epilogue {
   F16_STATS = 1,     // per row and 128 columns: (max, sum of 2^(l - max)) of l = (v + bias) log2 e; the target's l
   F16_DLOGITS = 2    // d = (2^((v + bias) log2 e - lse) - [column == target]) * coef, stored as an fp16 pair scaled by 2^15
 };
-constexpr float F16_D_SCALE = 32768.f;
+constexpr int F16_D_EXP = 15;
+constexpr float F16_D_SCALE = 32768.f;      // 2^F16_D_EXP
 
 struct F16Gemm {
   int64_t M = 0, N = 0, K = 0;
   HalfPair a, b;
-  const float *alpha_dev = nullptr;   // optional device scalar multiplied into v
+  const float *alpha_dev = nullptr;   // optional device scalar multiplied into v, and 2^alpha_exp
+  int alpha_exp = 0;
   const float *bias = nullptr;        // [N]
   // F16_STORE
   float *C = nullptr;
@@ -68,8 +70,8 @@ int launch_amax(const HalfJob &a, const HalfJob *b, cudaStream_t s);
 // The fp16 pairs of up to two arrays in one launch.
 int launch_half_split(const HalfJob &a, const HalfJob *b, cudaStream_t s);
 
-// out[n] = alpha (a device scalar, NULL: 1) times the sum of the rows of part [parts][N], in a fixed order.
-int launch_column_sums(const float *part, int parts, int64_t N, const float *alpha, float *out, cudaStream_t s);
+// out[n] = the sum of the rows of part [parts][N], in a fixed order, times scale, times alpha (a device scalar, NULL: 1).
+int launch_column_sums(const float *part, int parts, int64_t N, float scale, const float *alpha, float *out, cudaStream_t s);
 
 struct Carver {       // a caller's work space, handed out in 256-byte steps (base NULL: only measures)
   char *base;
@@ -81,15 +83,35 @@ struct Carver {       // a caller's work space, handed out in 256-byte steps (ba
   }
 };
 
-// Scale of an operand from its largest finite |x|: 2^(14 - floor(log2 amax)), at most 2^100, and its inverse.
+// Scale of an operand from its largest finite |x|: 2^(14 - floor(log2 amax)), at most 2^126 (an operand of
+// values below 2^-112 keeps fewer than 22 bits, down to those of a denormal), and its inverse.
 __host__ __device__ __forceinline__ int half_scale_exponent(uint32_t amax_bits) {
   if (amax_bits == 0) return 0;
   const int ex = 141 - (int)(amax_bits >> 23);
-  return ex > 100 ? 100 : ex;
+  return ex > 126 ? 126 : ex;
 }
 __device__ __forceinline__ float pow2f_exact(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }   // -126 <= e <= 127
 __device__ __forceinline__ float half_scale(const uint32_t *amax) { return amax ? pow2f_exact(half_scale_exponent(*amax)) : 1.f; }
-__device__ __forceinline__ float half_unscale(const uint32_t *amax) { return amax ? pow2f_exact(-half_scale_exponent(*amax)) : 1.f; }
+
+// A sum of scaled products is (sum * f0) * f1: the operands' unscaling, `alpha` (optional device scalar) and
+// 2^extra as two factors of about the same exponent, so that neither step leaves the range of fp32 unless
+// the result does.
+__device__ __forceinline__ void unscale_factors(const uint32_t *amax_a, const uint32_t *amax_b, const float *alpha, int extra,
+                                                float &f0, float &f1) {
+  int e = extra - (amax_a ? half_scale_exponent(*amax_a) : 0) - (amax_b ? half_scale_exponent(*amax_b) : 0);
+  float m = 1.f;
+  if (alpha) {
+    m = *alpha;
+    const int field = (int)(__float_as_uint(m) >> 23) & 0xFF;
+    if (field != 0 && field != 0xFF) {      // (zero, denormal, infinite or NaN: the value itself)
+      e += field - 127;
+      m = __uint_as_float((__float_as_uint(m) & 0x807FFFFFu) | 0x3F800000u);
+    }
+  }
+  const int e0 = e / 2, e1 = e - e0;
+  f0 = m * pow2f_exact(e0 < -126 ? -126 : (e0 > 126 ? 126 : e0));
+  f1 = pow2f_exact(e1 < -126 ? -126 : (e1 > 127 ? 127 : e1));
+}
 
 // hi and lo of a scaled value. An infinite or NaN value gives an infinite or NaN hi and a NaN lo.
 __device__ __forceinline__ void half_pair(float v, __half &hi, __half &lo) {

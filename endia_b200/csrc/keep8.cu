@@ -2,7 +2,7 @@
 //
 // Form: per row, blocks of 32 consecutive features share a power-of-two scale:
 //   x ~ q * 2^e,  e the smallest integer with round(max|x| / 2^e) <= 127,  q = round(x / 2^e) in [-127, 127]
-// (round half to even; e >= -126). 8.25 bits per value, an error of at most half of 2^e, which is between
+// (round half to even; -126 <= e <= 121, so that q * 2^e is finite: values beyond 127 * 2^121 become that). 8.25 bits per value, an error of at most half of 2^e, which is between
 // max/127.5/2 and max/63.75/2. With keep_sign a value that is not zero gets |q| >= 1, so that the
 // derivative of a ReLU taken from its kept output is the exact one. An infinite or NaN value is kept as
 // q = -128 and reads back as NaN; it does not count in the block's maximum.
@@ -85,13 +85,13 @@ keep8_kernel(const float *__restrict__ x, int64_t ld, int64_t rows, int64_t cols
       best = mx > best ? mx : best;
       // max / 2^e < 127.5: 127.5 = 64 * 1.9921875
       int e = (int)(mx >> 23) - 127 - 6 + ((mx & 0x7FFFFFu) >= 0x7F0000u ? 1 : 0);
-      e = e < -126 ? -126 : e;
+      e = e < -126 ? -126 : (e > 121 ? 121 : e);
       const float down = pow2f_exact(-e);
       uint32_t w[2] = {0u, 0u};
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const uint32_t b = __float_as_uint(v[f][u]) & 0x7FFFFFFFu;
-        int n = b < 0x7F800000u ? __float2int_rn(v[f][u] * down) : -128;
+        int n = b < 0x7F800000u ? max(-127, min(127, __float2int_rn(v[f][u] * down))) : -128;
         if (keep_sign && n == 0 && b != 0) n = v[f][u] < 0.f ? -1 : 1;
         w[u >> 2] |= ((uint32_t)n & 0xFFu) << (8 * (u & 3));
       }
@@ -393,7 +393,7 @@ int endia_b200_linear_keep_bwd(const void *kept_x, const float *W, int64_t ldw, 
   EB_LAUNCH_CHECK();
   ds_split_kernel<<<grid, 256, 0, s>>>(a, f.amax, f.dh, f.dl, f.ldd, db ? f.sums : nullptr);
   EB_LAUNCH_CHECK();
-  if (db && (st = launch_column_sums(f.sums, (int)ceil_div(M, 64), N, nullptr, db, s))) return st;
+  if (db && (st = launch_column_sums(f.sums, (int)ceil_div(M, 64), N, 1.f, nullptr, db, s))) return st;
   const Kept kx = kept_view(const_cast<void *>(kept_x), M, K);
   const HalfPair d{f.dh, f.dl, f.ldd, f.amax};
   if (dw) {

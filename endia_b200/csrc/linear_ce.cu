@@ -98,7 +98,7 @@ ce_rows_kernel(const float2 *__restrict__ stats, int parts, const float *__restr
 // The incoming gradient g as a row coefficient in [-1, 1] and one factor:
 //   scalar g (a sum or a mean): coef = 1, factor = g or g / count
 //   one g per row: coef = g_m / 2^e with 2^e >= max |g|, factor = 2^e
-// coef = 0: the row is left out; NaN: its target names no class. alpha = { factor, factor / 2^15 }.
+// coef = 0: the row is left out; NaN: its target names no class.
 __global__ void __launch_bounds__(1024)
 ce_coef_kernel(const float *__restrict__ g, int per_row, int mean, const float *__restrict__ count,
                const float *__restrict__ target, int M, int V, float *__restrict__ coef, float *__restrict__ alpha) {
@@ -115,16 +115,14 @@ ce_coef_kernel(const float *__restrict__ g, int per_row, int mean, const float *
     best = __reduce_max_sync(0xffffffffu, pm[threadIdx.x & 31]);
   }
   int e = best ? (int)(best >> 23) - 126 : 0;      // 2^e > max |g|
-  e = e < -100 ? -100 : (e > 120 ? 120 : e);
+  e = e > 126 ? 126 : e;
   const float down = pow2f_exact(-e);
   for (int m = threadIdx.x; m < M; m += 1024) {
     const float t = target[m];
     coef[m] = t < 0.f ? 0.f : (ce_invalid(t, V) ? NAN : (per_row ? g[m] * down : 1.f));
   }
   if (threadIdx.x == 0) {
-    const float f = per_row ? pow2f_exact(e) : (mean ? (count[0] > 0.f ? g[0] / count[0] : 0.f) : g[0]);
-    alpha[0] = f;
-    alpha[1] = f * (1.f / F16_D_SCALE);
+    alpha[0] = per_row ? pow2f_exact(e) : (mean ? (count[0] > 0.f ? g[0] / count[0] : 0.f) : g[0]);
   }
 }
 
@@ -266,7 +264,7 @@ static size_t ce_carve_backward(int64_t M, int64_t K, int64_t V, char *base, CeB
   Carver c{base};
   f = CeBackward{};
   f.coef = c.take<float>(M);
-  f.alpha = c.take<float>(2);
+  f.alpha = c.take<float>(1);
   f.amax = c.take<uint32_t>(2);
   f.piece = ce_piece(4 * (M + K), V);
   f.ldx = ceil_div(K, 8) * 8;
@@ -402,7 +400,7 @@ int endia_b200_linear_ce_bwd(const float *x, int64_t ldx, const float *W, int64_
       h.M = M; h.N = K; h.K = n;
       h.a = d;
       h.b = HalfPair{f.wh, f.wl, f.piece, amax + 1};
-      h.alpha_dev = f.alpha + 1;
+      h.alpha_dev = f.alpha; h.alpha_exp = -F16_D_EXP;
       h.C = dx; h.ldc = K; h.accumulate = v0 > 0; h.partial = f.partial;
       if ((st = launch_gemm_f16(h, false, false, F16_STORE, s))) return st;
     }
@@ -411,11 +409,11 @@ int endia_b200_linear_ce_bwd(const float *x, int64_t ldx, const float *W, int64_
       h.M = K; h.N = n; h.K = M;
       h.a = HalfPair{f.xh, f.xl, f.ldx, amax};
       h.b = d;
-      h.alpha_dev = f.alpha + 1;
+      h.alpha_dev = f.alpha; h.alpha_exp = -F16_D_EXP;
       h.C = dw + v0; h.ldc = V; h.partial = f.partial;
       if ((st = launch_gemm_f16(h, true, true, F16_STORE, s))) return st;
     }
-    if (db && (st = launch_column_sums(f.part_sums, (int)ceil_div(M, 32), n, f.alpha + 1, db + v0, s))) return st;
+    if (db && (st = launch_column_sums(f.part_sums, (int)ceil_div(M, 32), n, 1.f / F16_D_SCALE, f.alpha, db + v0, s))) return st;
   }
   return ENDIA_B200_OK;
 }

@@ -348,7 +348,7 @@ int endia_b200_linear_ce_bwd(const float *x, int64_t ldx, const float *W, int64_
 /* The 8-bit form of an array of `rows` x `cols` floats (leading dimension ldx) for a backward pass:
  * blocks of 32 consecutive columns share a power of two,
  *   x ~ q * 2^e,  e = the smallest integer >= -126 with round(max|x| / 2^e) <= 127,  q = round(x / 2^e)
- * (half to even). keep_sign != 0: a value that is not zero keeps |q| >= 1, so that the derivative of a
+ * (half to even; e is at most 121, and what lies beyond 127 * 2^121 becomes that). keep_sign != 0: a value that is not zero keeps |q| >= 1, so that the derivative of a
  * ReLU taken from its kept output is exact. Infinite and NaN values read back as NaN (and do not count
  * in max|x|). `kept` holds endia_b200_keep8_bytes(rows, cols) bytes (8.25 bits per value), 256-byte
  * aligned. keep8_read writes the values it stands for, contiguous [rows, cols]. */
