@@ -92,8 +92,13 @@ def flush_readers(dst):
 
 def compute_stride(shape):
     """Row-major element strides (endia/utils/_array_shape.mojo:24-30)."""
-    stride = [1] * len(shape)
-    for i in range(len(shape) - 2, -1, -1):
+    n = len(shape)
+    if n == 1:
+        return [1]
+    if n == 2:
+        return [shape[1], 1]
+    stride = [1] * n
+    for i in range(n - 2, -1, -1):
         stride[i] = stride[i + 1] * shape[i + 1]
     return stride
 
@@ -127,24 +132,26 @@ class Array:
     """Handle to a graph node with device storage. Constructor forms (as in the reference):
     Array([2, 3]) zeros of that shape; Array("[1, 2, 3]") literal; Array(numpy_array)."""
 
+    # What a node starts with (the lists are per node).
+    vjp_ = None
+    jvp_ = None
+    name = "arg"
+    grad_node = None
+    id = -1
+    is_view = False
+    base_ = None
+    buf = None
+
     def __init__(self, data=None, requires_grad=False, is_complex=False):
         self.args_ = []
-        self.vjp_ = None
-        self.jvp_ = None
-        self.name = "arg"
         self.meta_data = []
-        self.grad_node = None
-        self.id = -1
-        self.is_view = False
-        self.base_ = None
         self.requires_grad_flag = bool(requires_grad)
         self.is_complex_flag = bool(is_complex)
-        self.array_shape_ = ArrayShape([0])
-        self.buf = None
-        if data is None:
-            return
         if isinstance(data, ArrayShape):
             self.array_shape_ = data
+            return
+        self.array_shape_ = ArrayShape([0])
+        if data is None:
             return
         if isinstance(data, str):
             data = _parse_string(data)

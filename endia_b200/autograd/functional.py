@@ -3,7 +3,10 @@ grad / jacobian / hessian / value_and_grad (endia/autograd/functional.mojo:21-24
 branch of Callable.__call__, endia/compile/callable.mojo:100-197). The walk only enqueues kernels;
 nothing synchronises with the device."""
 from . import state as _state
-from ..utils.general import top_order, reset_node_id_recursive, remove_grad_rec
+from ..functional.binary_ops import add
+from ..functional.init_ops import ones, eye
+from ..functional.view_ops import reshape
+from ..utils.general import top_order, remove_grad_rec
 
 
 def backward(arg, create_graph=False):
@@ -22,9 +25,6 @@ def jacrev(arg, create_graph=False, only_for=None):
     shape out.shape + out.shape, so the stored gradients are full Jacobians (:34-38). Gradients
     ACCUMULATE into nodes that already hold one (:55-57). Unless `create_graph`, the graph edges of
     each new gradient are cut (:63-65)."""
-    from ..functional.init_ops import ones, eye
-    from ..functional.view_ops import reshape
-    from ..functional.binary_ops import add
     out = arg
     trace = top_order(out)
     wanted = None
@@ -77,7 +77,8 @@ def jacrev(arg, create_graph=False, only_for=None):
     finally:
         _state.create_graph = prev
         _state.grad_wanted = prev_wanted
-        reset_node_id_recursive(out)
+        for node in trace:
+            node.id = -1
 
 
 def jvp(out, inputs, tangents):

@@ -129,7 +129,7 @@ ce_coef_kernel(const float *__restrict__ g, int per_row, int mean, const float *
 // ------------------------------------------------------------------------------------ few rows, fp32
 // The statistics of up to 16 rows in one pass over W, which is all that such a call has to read: a CTA takes 128
 // columns, its eight warps take the features in turn (x as [feature][row] in shared memory, four columns
-// and ROWS x 4 sums a lane), and eight loads of 128 bits a lane are in flight. The warps' sums are added in
+// and ROWS x 4 sums a lane), and eight to sixteen loads of 128 bits a lane are in flight. The warps' sums are added in
 // order, then a warp per row (two rows) reduces 128 logits as the tensor-core epilogue does.
 constexpr int CE_FEW = 16, CE_FEW_K = 512;
 template <int ROWS, bool VEC>
@@ -158,8 +158,8 @@ ce_few_rows_kernel(const float *__restrict__ x, int64_t ldx, const float *__rest
       xs[k][r] = r < M ? __ldg(x + (int64_t)r * ldx + k0 + k) : 0.f;
     }
     __syncthreads();
-    for (int kb = w; kb < kn; kb += 64) {
-      float v[8][4];
+    // features kb, kb + 8, ... kb + 56 of this warp; the next eight are in flight while these are used
+    auto load = [&](float (&v)[8][4], int kb) {
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const int k = kb + 8 * u;
@@ -172,6 +172,8 @@ ce_few_rows_kernel(const float *__restrict__ x, int64_t ldx, const float *__rest
           for (int j = 0; j < 4; ++j) v[u][j] = k < kn && col[j] < V ? __ldcs(row + col[j]) : 0.f;
         }
       }
+    };
+    auto use = [&](const float (&v)[8][4], int kb) {
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const int k = kb + 8 * u;
@@ -184,6 +186,14 @@ ce_few_rows_kernel(const float *__restrict__ x, int64_t ldx, const float *__rest
           }
         }
       }
+    };
+    float va[8][4], vb[8][4];
+    load(va, w);
+    for (int kb = w; kb < kn; kb += 128) {
+      load(vb, kb + 64);
+      use(va, kb);
+      load(va, kb + 128);
+      use(vb, kb + 64);
     }
   }
   for (int src = 0; src < 8; ++src) {

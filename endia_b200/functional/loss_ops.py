@@ -4,7 +4,7 @@ from .. import _lib
 from .._array import Array, ArrayShape, alloc, stream
 from ..autograd import state as _state
 from ._utils import op_array, setup_shape_and_data, contiguous
-from .binary_ops import sub, mul, add, fused_binary
+from .binary_ops import sub, mul, add, fused_binary, _matrix_layout
 from .reduce_ops import sum
 
 
@@ -63,11 +63,12 @@ _REDUCTIONS = {"mean": _lib.LOSS_MEAN, "sum": _lib.LOSS_SUM, "none": _lib.LOSS_N
 
 def _row_major(a):
     """`a` (2-D) itself when its rows are contiguous runs, else a contiguous copy, and its leading dimension."""
-    from .binary_ops import _matrix_layout
+    if a.is_contiguous():
+        return a, max(a.shape()[1], 1)
     layout = _matrix_layout(a)
     if layout is None or layout[0] != 0:
         a = contiguous(a)
-        layout = (0, max(a.shape()[1], 1))
+        return a, max(a.shape()[1], 1)
     return a, layout[1]
 
 

@@ -9,7 +9,8 @@ from ..functional import init_ops
 from ..functional._utils import op_array, setup_shape_and_data, contiguous
 from ..functional.binary_ops import matmul, mul, add, gemm_arrays
 from ..functional.comparison_ops import greater
-from ..functional.keep_ops import keep8
+from ..functional.keep_ops import Kept8, keep8, keeps_sign
+from ..functional.loss_ops import _row_major, _scratch
 from ..functional.reduce_ops import reduce_add
 from ..functional.unary_ops import relu, tanh, sigmoid, square
 
@@ -198,8 +199,6 @@ def _linear_kept(x, weight, bias, act):
     activation's derivative; exact for ReLU). x itself stays as it is: keep8(x) releases its float32
     storage once nothing else needs it. With create_graph=True the VJP is the composition of
     differentiable ops, on whatever x and out then hold."""
-    from ..functional.keep_ops import Kept8, quantise, keeps_sign
-    from ..functional.loss_ops import _row_major, _scratch
     if x.ndim() != 2 or weight.ndim() != 2 or (bias is not None and bias.ndim() != 1) or \
             any(a.is_complex() for a in [x, weight] + ([bias] if bias is not None else [])):
         raise _lib.EndiaError(_lib.EINVAL, "linear: checkpoint=True takes real arrays x (B, K), weight (K, N), bias (N)")

@@ -3,7 +3,8 @@ a torch tensor element by element; here the storage is shared or copied in one t
 import numpy as np
 import torch
 
-from .._array import Array, ArrayShape
+from .. import _lib
+from .._array import Array, ArrayShape, alloc, device
 
 
 def to_torch(arg, copy=True):
@@ -32,20 +33,17 @@ def from_torch(t, requires_grad=None, copy=True):
     src = t.detach()
     is_c = src.is_complex()
     if not copy:
-        from .. import _lib
-        from .._array import device
         if src.device != device() or src.dtype not in (torch.float32, torch.complex64) or not src.is_contiguous():
             raise _lib.EndiaError(_lib.EINVAL, "from_torch: copy=False needs a contiguous float32 or complex64 tensor on %s"
                                   % device())
         out = Array(ArrayShape(list(src.shape) if src.dim() else [1]))
         out.is_complex_flag = is_c
-        out.buf = (torch.view_as_real(src) if is_c else src).reshape(-1)
+        out.buf = (torch.view_as_real(src) if is_c else src).view(-1)
         out.requires_grad_flag = bool(t.requires_grad if requires_grad is None else requires_grad)
         return out
     src = src.to(torch.complex64 if is_c else torch.float32).contiguous()
     out = Array(ArrayShape(list(src.shape) if src.dim() else [1]))
     out.is_complex_flag = is_c
-    from .._array import alloc, device
     flat = (torch.view_as_real(src) if is_c else src).reshape(-1)
     out.buf = alloc(flat.numel())
     if flat.numel():
