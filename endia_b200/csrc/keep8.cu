@@ -8,7 +8,7 @@
 // q = -128 and reads back as NaN; it does not count in the block's maximum.
 // Why a power of two: x / 2^e and q * 2^e are exact in fp32, and q * 2^e is exact in fp16 after one scale
 // for the whole array, so the weight gradient h^T ds needs two fp16 products instead of three.
-// Layout: a head of 256 bytes ([0]: bits of the largest finite |x|), q [rows][cols rounded up to 32],
+// Layout: a head of 256 bytes ([0]: bits of the largest finite |x|, [1]: scratch of the layer), q [rows][cols rounded up to 32],
 // e + 127 [rows][cols / 32 rounded up] as bytes.
 //
 // The layer: out = act(x W + b) from x itself; for its backward pass only the kept forms are read:
@@ -39,10 +39,9 @@ __host__ __device__ static inline Kept kept_view(void *p, int64_t rows, int64_t 
   return k;
 }
 
-// 4 lanes per block of 32, eight values each (128-bit loads where VEC); two blocks per lane group in flight.
-template <bool VEC>
-__device__ __forceinline__ void keep_load(const float *src, int64_t left, float (&v)[8]) {
-  if (VEC && left >= 8) {
+// 4 lanes per block of 32, eight values each (128-bit loads where `vec`); two blocks per lane group in flight.
+__device__ __forceinline__ void ld8(const float *src, int64_t left, bool vec, float (&v)[8]) {
+  if (vec && left >= 8) {
     const float4 a = __ldg(reinterpret_cast<const float4 *>(src)), b = __ldg(reinterpret_cast<const float4 *>(src) + 1);
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   } else {
@@ -50,9 +49,8 @@ __device__ __forceinline__ void keep_load(const float *src, int64_t left, float 
     for (int u = 0; u < 8; ++u) v[u] = u < left ? __ldg(src + u) : 0.f;
   }
 }
-template <bool VEC>
 __global__ void __launch_bounds__(256)
-keep8_kernel(const float *__restrict__ x, int64_t ld, int64_t rows, int64_t cols, int keep_sign, Kept k) {
+keep8_kernel(const float *__restrict__ x, int64_t ld, int64_t rows, int64_t cols, int keep_sign, bool vec, Kept k) {
   constexpr int IN_FLIGHT = 2;
   const int64_t per_row = k.ldq / 8, total = rows * per_row, step = (int64_t)gridDim.x * blockDim.x;
   const bool narrow = total < ((int64_t)1 << 31);
@@ -67,7 +65,7 @@ keep8_kernel(const float *__restrict__ x, int64_t ld, int64_t rows, int64_t cols
       const bool in = i < total;
       row[f] = !in ? -1 : (narrow ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row);
       col[f] = in ? (i - row[f] * per_row) * 8 : 0;
-      keep_load<VEC>(x + (in ? row[f] * ld : 0) + col[f], in ? cols - col[f] : 0, v[f]);
+      ld8(x + (in ? row[f] * ld : 0) + col[f], in ? cols - col[f] : 0, vec, v[f]);
     }
 #pragma unroll
     for (int f = 0; f < IN_FLIGHT; ++f) {
@@ -170,31 +168,28 @@ struct DsArgs {
 __device__ __forceinline__ void ds8(const DsArgs &a, int64_t r, int64_t c, float (&v)[8]) {
   const int64_t left = a.N - c;
   float o[8];
-  auto load = [&](const float *p, float (&t)[8]) {
-    if (a.vec && left >= 8) {
-      const float4 x = __ldg(reinterpret_cast<const float4 *>(p)), y = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-      t[0] = x.x; t[1] = x.y; t[2] = x.z; t[3] = x.w; t[4] = y.x; t[5] = y.y; t[6] = y.z; t[7] = y.w;
-    } else {
-#pragma unroll
-      for (int u = 0; u < 8; ++u) t[u] = u < left ? __ldg(p + u) : 0.f;
-    }
-  };
-  load(a.g + r * a.N + c, v);
+  ld8(a.g + r * a.N + c, left, a.vec, v);
   if (a.act) {
-    if (a.out) load(a.out + r * a.N + c, o);
+    if (a.out) ld8(a.out + r * a.N + c, left, a.vec, o);
     else kept8(a.kept, r, c, 1.f, o);
 #pragma unroll
     for (int u = 0; u < 8; ++u) v[u] = u < left ? v[u] * act_bwd(a.act, o[u]) : 0.f;
   }
 }
-__global__ void __launch_bounds__(256) ds_amax_kernel(DsArgs a, uint32_t *__restrict__ amax) {
-  const int64_t per_row = (a.N + 7) / 8, total = a.M * per_row, step = (int64_t)gridDim.x * blockDim.x;
+// The largest finite |ds| and, in the CTAs from `split` on, the largest finite |W|.
+__global__ void __launch_bounds__(256) ds_amax_kernel(DsArgs a, const float *__restrict__ W, int64_t w_rows, int64_t w_cols, int64_t ldw,
+                                                      int split, uint32_t *__restrict__ amax) {
+  const bool second = (int)blockIdx.x >= split;
+  const int block = (int)blockIdx.x - (second ? split : 0), blocks = second ? (int)gridDim.x - split : split;
+  const int64_t per_row = ((second ? w_cols : a.N) + 7) / 8, total = (second ? w_rows : a.M) * per_row, step = (int64_t)blocks * blockDim.x;
   const bool narrow = total < ((int64_t)1 << 31);
+  const bool vec = ldw % 4 == 0 && (reinterpret_cast<uintptr_t>(W) & 15) == 0;
   uint32_t best = 0;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
+  for (int64_t i = (int64_t)block * blockDim.x + threadIdx.x; i < total; i += step) {
     const int64_t r = narrow ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row, c = (i - r * per_row) * 8;
     float v[8];
-    ds8(a, r, c, v);
+    if (second) ld8(W + r * ldw + c, w_cols - c, vec, v);
+    else ds8(a, r, c, v);
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const uint32_t b = __float_as_uint(v[u]) & 0x7FFFFFFFu;
@@ -202,7 +197,7 @@ __global__ void __launch_bounds__(256) ds_amax_kernel(DsArgs a, uint32_t *__rest
     }
   }
   best = __reduce_max_sync(0xffffffffu, best);
-  if ((threadIdx.x & 31) == 0 && best) atomicMax(amax, best);
+  if ((threadIdx.x & 31) == 0 && best) atomicMax(amax + (second ? 1 : 0), best);
 }
 // The fp16 pair of ds and its sums over 64 rows: a CTA takes 64 rows x 128 columns.
 __global__ void __launch_bounds__(256)
@@ -289,8 +284,7 @@ static int run_keep8(const float *x, int64_t ld, int64_t rows, int64_t cols, int
   const Kept k = kept_view(kept, rows, cols);
   const int grid = grid_for(rows * (k.ldq / 8), 256, 8);
   const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ld % 4 == 0 || rows == 1);
-  if (vec) keep8_kernel<true><<<grid, 256, 0, s>>>(x, ld, rows, cols, keep_sign, k);
-  else keep8_kernel<false><<<grid, 256, 0, s>>>(x, ld, rows, cols, keep_sign, k);
+  keep8_kernel<<<grid, 256, 0, s>>>(x, ld, rows, cols, keep_sign, vec, k);
   EB_LAUNCH_CHECK();
   return ENDIA_B200_OK;
 }
@@ -349,17 +343,17 @@ int endia_b200_linear_keep_fwd(const float *x, int64_t ldx, const float *W, int6
   if (N == 0) return ENDIA_B200_OK;
   KeepForward f;
   keep_carve_forward(M, N, K, static_cast<char *>(scratch), f);
-  EB_CUDA(cudaMemsetAsync(f.amax, 0, 2 * sizeof(uint32_t), s));
-  // the 8-bit form has found the largest |x| already
-  uint32_t *amax_x = kept_x ? static_cast<uint32_t *>(kept_x) : f.amax;
-  HalfJob jw{W, K, N, ldw, nullptr, f.amax + 1, f.wh, f.wl, f.ldw};
+  // the 8-bit form has found the largest |x| already; its head, cleared with it, has room for W's
+  uint32_t *amax_x = kept_x ? static_cast<uint32_t *>(kept_x) : f.amax, *amax_w = amax_x + 1;
+  if (!kept_x) EB_CUDA(cudaMemsetAsync(f.amax, 0, 2 * sizeof(uint32_t), s));
+  HalfJob jw{W, K, N, ldw, nullptr, amax_w, f.wh, f.wl, f.ldw};
   HalfJob jx{x, M, K, ldx, nullptr, amax_x, f.xh, f.xl, f.ldx};
   if ((st = launch_amax(jw, kept_x ? nullptr : &jx, s))) return st;
   if ((st = launch_half_split(jw, &jx, s))) return st;
   F16Gemm g;
   g.M = M; g.N = N; g.K = K;
   g.a = HalfPair{f.xh, f.xl, f.ldx, amax_x};
-  g.b = HalfPair{f.wh, f.wl, f.ldw, f.amax + 1};
+  g.b = HalfPair{f.wh, f.wl, f.ldw, amax_w};
   g.bias = bias; g.act = act; g.C = out; g.ldc = N; g.partial = f.partial;
   return launch_gemm_f16(g, false, true, F16_STORE, s);
 }
@@ -389,7 +383,8 @@ int endia_b200_linear_keep_bwd(const void *kept_x, const float *W, int64_t ldw, 
   a.vec = N % 4 == 0 && (reinterpret_cast<uintptr_t>(grad) & 15) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
   const dim3 grid((unsigned)ceil_div(N, 128), (unsigned)(ceil_div(M, 64) < 32768 ? ceil_div(M, 64) : 32768));
   EB_CUDA(cudaMemsetAsync(f.amax, 0, 2 * sizeof(uint32_t), s));
-  ds_amax_kernel<<<grid_for(M * ceil_div(N, 8), 256, 8), 256, 0, s>>>(a, f.amax);
+  const int split = grid_for(M * ceil_div(N, 8), 256, 8), more = dx ? grid_for(K * ceil_div(N, 8), 256, 8) : 0;
+  ds_amax_kernel<<<split + more, 256, 0, s>>>(a, W, K, N, ldw, split, f.amax);
   EB_LAUNCH_CHECK();
   ds_split_kernel<<<grid, 256, 0, s>>>(a, f.amax, f.dh, f.dl, f.ldd, db ? f.sums : nullptr);
   EB_LAUNCH_CHECK();
@@ -408,7 +403,6 @@ int endia_b200_linear_keep_bwd(const void *kept_x, const float *W, int64_t ldw, 
   }
   if (dx) {
     const HalfJob jw{W, K, N, ldw, nullptr, f.amax + 1, f.wh, f.wl, f.ldw};
-    if ((st = launch_amax(jw, nullptr, s))) return st;
     if ((st = launch_half_split(jw, nullptr, s))) return st;
     F16Gemm g;
     g.M = M; g.N = K; g.K = N;

@@ -180,19 +180,18 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean"):
         return sub(div(e, reduce_add(e, [1])), equal(reshape(labels, [M, 1]), _class_numbers(V)))
 
     def vjp(primals, grad, out):
-        zero = Array(0)
         want = [_state.wants_grad(p) for p in primals]
         if _state.create_graph:
             from .binary_ops import matmul
             from .reduce_ops import reduce_add
             d = mul(errors(primals), row_weights(grad))
-            res = [matmul(d, primals[1].T()) if want[0] else zero, matmul(primals[0].T(), d) if want[1] else zero]
+            res = [matmul(d, primals[1].T()) if want[0] else None, matmul(primals[0].T(), d) if want[1] else None]
             if bias is not None:
-                res.append(reduce_add(d, [0]) if want[2] else zero)
+                res.append(reduce_add(d, [0]) if want[2] else None)
             return res
         res = []
         for w, shape in zip(want, ([M, K], [K, V], [1, V])):
-            res.append(zero)
+            res.append(None)
             if w:
                 res[-1] = Array(ArrayShape(shape))
                 setup_shape_and_data(res[-1])

@@ -227,17 +227,16 @@ def _linear_kept(x, weight, bias, act):
 
     def vjp(primals, grad, out):
         xp, wp = primals[0], primals[1]
-        zero = Array(0)
         want = [_state.wants_grad(p) for p in primals]
         if _state.create_graph:
             ds = _act_bwd_graph(act, out, grad)
-            res = [matmul(ds, wp.T()) if want[0] else zero, matmul(xp.T(), ds) if want[1] else zero]
+            res = [matmul(ds, wp.T()) if want[0] else None, matmul(xp.T(), ds) if want[1] else None]
             if bias is not None:
-                res.append(reduce_add(ds, [0]) if want[2] else zero)
+                res.append(reduce_add(ds, [0]) if want[2] else None)
             return res
         res = []
         for w, shape in zip(want, ([B, K], [K, N], [1, N])):      # (bias gradient: kept dim, like Expand.vjp)
-            res.append(zero)
+            res.append(None)
             if w:
                 res[-1] = Array(ArrayShape(shape))
                 setup_shape_and_data(res[-1])
