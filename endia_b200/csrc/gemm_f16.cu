@@ -4,7 +4,7 @@
 // product, but with another division of the work, because what limits accuracy there is the
 // accumulator: tensor memory adds with rounding toward zero, a bias that grows with the number of
 // adds (1e-5 of the result after 2048 of K). Here an accumulator lives for one stage of 64 of K (two in
-// the logit kernels, see f16_run_first):
+// some kernels, see f16_run_first):
 //   - the eight correction MMAs first, into an empty accumulator (they are 2^-11 of the result, so
 //     their truncation is too), then the four MMAs of hi*hi: four truncating adds in all;
 //   - the epilogue warps add it to the tile's sums, which they hold in registers (128 a thread) with
@@ -71,16 +71,19 @@ __device__ __forceinline__ void f16_load(uint32_t dst, const CUtensorMap *map, u
   }
 }
 
-// A run: the stages that one accumulator sums before it is drained. Stage i of a tile of n is the first
-// or the last of its run. Products that are stored have runs of one stage. The logit kernels have runs
-// of two: their epilogue (exponentials of a whole tile) outlasts the two stages that the MMAs can run
-// ahead with runs of one (2048 x 1024 x 32768: statistics 294 -> 262 us, d 177 -> 162 us; a stored
-// product gains nothing). Expected loss to truncation, 4.3e-8 of the running sum per add: 1.1e-7 of the
-// result with runs of one, 3.7e-7 with runs of two (the second stage's corrections add to the full sum).
-template <int EPI>
-__device__ __forceinline__ bool f16_run_first(int i) { return EPI == F16_STORE || (i & 1) == 0; }
-template <int EPI>
-__device__ __forceinline__ bool f16_run_last(int i, int n) { return EPI == F16_STORE || (i & 1) == 1 || i == n - 1; }
+// A run: the stages that one accumulator sums before it is drained; stage i of a tile of n is the first
+// or the last of its run. Stored products of two pairs have runs of one stage. Runs of two:
+//   - the logit kernels: their epilogue (exponentials of a whole tile) outlasts the two stages that the MMAs can
+//     run ahead with runs of one (2048 x 1024 x 32768: statistics 294 -> 262 us, d 177 -> 162 us)
+//   - products with an exact operand: a stage is 1024 cycles of MMAs there, shorter than a drain and its
+//     hand-over (layer 8192 x 4096 x 4096, the whole step: 2.22 -> 2.18 ms)
+// Expected loss to truncation, 4.3e-8 of the running sum per add: 1.1e-7 of the result with runs of one,
+// 3.7e-7 (2.8e-7 with an exact operand) with runs of two, where the second stage's corrections add to the
+// full sum. A stored product of two pairs gains 1 to 2 % from runs of two and keeps the smaller error.
+template <int PROD, int EPI>
+__device__ __forceinline__ bool f16_run_first(int i) { return (PROD == 3 && EPI == F16_STORE) || (i & 1) == 0; }
+template <int PROD, int EPI>
+__device__ __forceinline__ bool f16_run_last(int i, int n) { return (PROD == 3 && EPI == F16_STORE) || (i & 1) == 1 || i == n - 1; }
 
 // Column sums over a warp's 32 rows: v[j] of lane r is row r, column j; returns, in lane L, the sum of
 // column L. Halves the columns a lane is responsible for in each of five exchanges.
@@ -208,7 +211,7 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
         k_range(t, kb0, kb1);
         const int n = kb1 - kb0;
         for (int i = 0; i < n; ++i) {
-          const bool first = f16_run_first<EPI>(i), last = f16_run_last<EPI>(i, n);
+          const bool first = f16_run_first<PROD, EPI>(i), last = f16_run_last<PROD, EPI>(i, n);
           const uint32_t b = j & 1;
           if (!mbar_wait(full_bar((int)s), s_phase, 54)) { ok = false; break; }
           if (first && j >= 2 && !mbar_wait(acc_empty((int)b), ((j >> 1) - 1) & 1, 53)) { ok = false; break; }
@@ -256,7 +259,7 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
 #pragma unroll
       for (int i = 0; i < 128; ++i) acc[i] = 0.f;
       for (int i = 0, n = kb1 - kb; i < n; ++i) {
-        if (!f16_run_last<EPI>(i, n)) continue;
+        if (!f16_run_last<PROD, EPI>(i, n)) continue;
         const uint32_t b = j & 1;
         if (!mbar_wait(acc_full((int)b), (j >> 1) & 1, 55)) { ok = false; break; }
         tc_fence_after();
