@@ -83,6 +83,8 @@ int launch_splitk_finish(const GemmParams &p, int splits, cudaStream_t s);
 bool tc_gemm_supported(const GemmParams &p, int trans_a, int trans_b, int64_t batch,
                        bool explicit_request);
 int launch_gemm_tc(const GemmParams &p, int trans_a, int trans_b, cudaStream_t s, bool *c16_written = nullptr);
+// CTA pairs that the persistent two-CTA kernels may fill (SM pairs minus the reserve for concurrent kernels).
+int pair_capacity();
 // Scheme GEMM_AUTO uses on the two-CTA kernel (1 unless ENDIA_B200_TC_SCHEME=3xtf32).
 int tc_default_scheme();
 

@@ -656,7 +656,7 @@ bool gemm_f16_available() { return encode_fn() != nullptr; }
 // Ranges of K of an F16_STORE product: when its tiles leave half of the CTA pairs idle, each tile's
 // reduction is cut into up to 16 ranges of at least 512.
 static int k_ranges(int64_t M, int64_t N, int64_t K) {
-  const int64_t tiles = ceil_div(M, 256) * ceil_div(N, 256), cap = (sm_count() > 0 ? sm_count() : 148) / 2;
+  const int64_t tiles = ceil_div(M, 256) * ceil_div(N, 256), cap = pair_capacity();
   if (2 * tiles > cap) return 1;
   int64_t sp = cap / tiles;
   if (sp > K / 512) sp = K / 512;
@@ -690,7 +690,7 @@ static int launch_kernel(const F16Maps &maps, const F16Params &p, cudaStream_t s
       cudaGetLastError();
       nc = (sm_count() > 0 ? sm_count() : 148) / 2;
     }
-    max_pairs = nc;
+    max_pairs = nc < pair_capacity() ? nc : pair_capacity();
   }
   const int items = p.pairs_m * p.tiles_n * p.ksplit, pairs = items < max_pairs ? items : max_pairs;
   kern<<<dim3((unsigned)(2 * pairs)), F16_THREADS, SMEM, s>>>(maps, p);

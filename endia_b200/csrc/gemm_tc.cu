@@ -1046,7 +1046,7 @@ static bool pair_split_mode() {
 }
 
 // CTA pairs the persistent kernel runs with (SM pairs minus the reserve for concurrent kernels).
-static int pair_capacity() {
+int pair_capacity() {
   static const int cap = []() {
     const int sms = sm_count() > 0 ? sm_count() : 148;
     const char *rs = getenv("ENDIA_B200_TC_RESERVE_SMS");

@@ -102,8 +102,8 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean"):
 
     A negative target leaves its row out: loss 0, no gradient, whatever x holds there; a mean over no
     rows is 0. A target that is not an integer below V makes its row's loss NaN, and with it the
-    gradients. The target takes no gradient. With create_graph=True (and in forward mode) the VJP is the
-    differentiable composition of the same formula, which does hold logits, and wants finite x and
+    gradients. The target takes no gradient. With create_graph=True (and in forward mode, and for the
+    Jacobian of the row losses) the VJP is the differentiable composition of the same formula, which does hold logits, and wants finite x and
     valid targets in every row. The reference has mse only (loss_ops/mse_op.mojo:18-20)."""
     if reduction not in _REDUCTIONS:
         raise _lib.EndiaError(_lib.EINVAL, "linear_cross_entropy: unknown reduction %r" % (reduction,))
@@ -157,8 +157,9 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean"):
         from .comparison_ops import greater_equal, equal
         from .view_ops import reshape
         counted = greater_equal(reshape(labels, [M, 1]), Array([1]))
-        if mode == _lib.LOSS_NONE:
-            return mul(counted, reshape(contiguous(grad), [M, 1]))
+        if mode == _lib.LOSS_NONE:      # (leading dims of a Jacobian's seed stay in front)
+            lead = grad.shape()[:grad.ndim() - target.ndim()]
+            return mul(counted, reshape(contiguous(grad), lead + [M, 1]))
         if mode == _lib.LOSS_MEAN:
             from .binary_ops import div
             count = state_array([1], 0)
@@ -181,13 +182,13 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean"):
 
     def vjp(primals, grad, out):
         want = [_state.wants_grad(p) for p in primals]
-        if _state.create_graph:
+        if _state.create_graph or grad.shape() != out.shape():
             from .binary_ops import matmul
             from .reduce_ops import reduce_add
             d = mul(errors(primals), row_weights(grad))
             res = [matmul(d, primals[1].T()) if want[0] else None, matmul(primals[0].T(), d) if want[1] else None]
             if bias is not None:
-                res.append(reduce_add(d, [0]) if want[2] else None)
+                res.append(reduce_add(d, [-2]) if want[2] else None)
             return res
         res = []
         for w, shape in zip(want, ([M, K], [K, V], [1, V])):

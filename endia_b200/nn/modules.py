@@ -219,7 +219,8 @@ def _linear_kept(x, weight, bias, act):
         kept = None
         if curr.requires_grad_flag:
             kept = saved["x"] = alloc((_lib.lib.endia_b200_keep8_bytes(B, K) + 3) // 4)
-            a[0]._kept8 = kept
+            if a[0].args_:
+                a[0]._kept8 = kept      # (for keep8; a leaf's storage may be rewritten, it is not remembered)
         scratch = _scratch(_lib.lib.endia_b200_linear_keep_scratch_bytes(B, N, K, 0))
         _lib.call("endia_b200_linear_keep_fwd", xr.data_ptr(), ldx, wr.data_ptr(), ldw,
                   b.data_ptr() if b is not None else None, act, B, N, K, curr.data_ptr(),
@@ -228,11 +229,11 @@ def _linear_kept(x, weight, bias, act):
     def vjp(primals, grad, out):
         xp, wp = primals[0], primals[1]
         want = [_state.wants_grad(p) for p in primals]
-        if _state.create_graph:
+        if _state.create_graph or grad.shape() != out.shape():      # (a Jacobian's seed has dims in front)
             ds = _act_bwd_graph(act, out, grad)
             res = [matmul(ds, wp.T()) if want[0] else None, matmul(xp.T(), ds) if want[1] else None]
             if bias is not None:
-                res.append(reduce_add(ds, [0]) if want[2] else None)
+                res.append(reduce_add(ds, [-2]) if want[2] else None)
             return res
         res = []
         for w, shape in zip(want, ([B, K], [K, N], [1, N])):      # (bias gradient: kept dim, like Expand.vjp)

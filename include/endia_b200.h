@@ -330,7 +330,7 @@ enum { ENDIA_B200_LOSS_MEAN = 0, ENDIA_B200_LOSS_SUM = 1, ENDIA_B200_LOSS_NONE =
  *   dx [M, K], dw [K, V], db [V], all contiguous, each may be NULL (not computed)
  * `scratch`: endia_b200_linear_ce_scratch_bytes(M, K, V, backward) bytes, 256-byte aligned: the
  * vocabulary is walked in equal pieces whose work space stays near 256 MiB (pieces of at least 1024
- * columns). Limits: V <= 2^24 (class numbers are float32 values), M and K below 2^27. The order of
+ * columns), beside 4 bytes per element of x and, forward, 8 bytes per row and 128 classes. Limits: V <= 2^24 (class numbers are float32 values), M and K below 2^27. The order of
  * every sum is fixed: the same inputs give the same bits.
  * Accuracy: products of 22-bit operand pairs summed in fp32 (fp32 kernels for small problems).
  * No counterpart in the reference, whose one loss is mse (endia/functional/loss_ops/mse_op.mojo:18-20). */

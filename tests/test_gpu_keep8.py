@@ -315,6 +315,34 @@ def test_second_order_through_a_checkpointed_layer(nd):
     assert np.abs(dw - want).max() <= 1e-4 * np.abs(want).max()
 
 
+def test_jacobian_of_a_checkpointed_layer(nd):
+    x, w, b, _ = layer_case(3, 5, 4, 21)
+    X, W, B = (nd.Array(a, requires_grad=True) for a in (x, w, b))
+    nd.nn.linear(X, W, B, "tanh", checkpoint=True).backward()
+    y = np.tanh(x.astype(np.float64) @ w + b)
+    jx = np.einsum("in,kn,ij->injk", 1 - y * y, w, np.eye(3))
+    jw = np.einsum("in,ik,nm->inkm", 1 - y * y, x, np.eye(4))
+    jb = np.einsum("in,nm->inm", 1 - y * y, np.eye(4))
+    assert np.abs(X.grad().to_numpy() - jx).max() <= 1e-5
+    assert np.abs(W.grad().to_numpy() - jw).max() <= 1e-5
+    assert np.abs(B.grad().to_numpy()[:, :, 0] - jb).max() <= 1e-5
+
+
+def test_an_input_batch_is_not_remembered(nd):
+    """The layer's 8-bit copy of a leaf goes with the graph: the leaf holds nothing of it."""
+    x, w, b, g = layer_case(2000, 512, 16, 22)
+    X, W = nd.Array(x), nd.Array(w, requires_grad=True)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    out = nd.nn.linear(X, W, checkpoint=True)
+    held = torch.cuda.memory_allocated() - before
+    assert held >= 2000 * 512
+    del out
+    import gc
+    gc.collect()
+    assert torch.cuda.memory_allocated() - before < 2000 * 512
+
+
 def test_nan_and_infinite_activations(nd):
     """A row with a NaN or an infinity spoils the weight gradient's rows that it reaches and no other row of dx."""
     x, w, b, g = layer_case(40, 33, 34, 13)

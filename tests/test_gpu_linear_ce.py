@@ -407,6 +407,21 @@ def test_second_order_and_forward_mode(nd):
     assert tan.shape() == [M] and tan.to_numpy()[2] == 0
 
 
+def test_jacobian_of_the_row_losses(nd):
+    M, K, V = 5, 6, 9
+    x, w, b, t = inputs(M, K, V, seed=28)
+    t[1] = -1
+    X, W, B = (nd.Array(a, requires_grad=True) for a in (x, w, b))
+    rows = nd.linear_cross_entropy(X, W, nd.Array(t), bias=B, reduction="none")
+    rows.backward()
+    assert X.grad().shape() == [M, M, K] and W.grad().shape() == [M, K, V]
+    for i in range(M):
+        ref, _ = formula(x, w, t, b, np.eye(M)[i])
+        assert np.abs(X.grad().to_numpy()[i] - ref["dx"].cpu().numpy()).max() <= 1e-5
+        assert np.abs(W.grad().to_numpy()[i] - ref["dw"].cpu().numpy()).max() <= 1e-5
+        assert np.abs(B.grad().to_numpy()[i, 0] - ref["db"].cpu().numpy()).max() <= 1e-5
+
+
 def test_on_another_stream(nd):
     x, w, b, t = inputs(200, 64, 3000, seed=27)
     want = step(nd, x, w, t, b, "mean")
