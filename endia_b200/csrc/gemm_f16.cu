@@ -39,7 +39,9 @@ struct F16Maps {
 struct F16Params {
   int M, N;
   int pairs_m, tiles_n, group_m, ksplit, nkb;   // nkb: stages of 64 of K in all
-  const uint32_t *amax_a, *amax_b;
+  const int *ea, *eb;            // the operands' scale exponents, leading dimensions and last blocks along m and n
+  int64_t ea_ld, eb_ld;
+  int a_last, b_last;
   const float *alpha_dev;
   int alpha_exp;
   const float *bias;
@@ -128,10 +130,11 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
   const bool leader = rank == 0;
   const int num_pairs = (int)(gridDim.x >> 1), pair_id = (int)(blockIdx.x >> 1);
   const int tiles_mn = p.pairs_m * p.tiles_n, num_items = tiles_mn * p.ksplit;
-  auto k_range = [&](int t, int &kb0, int &kb1) {      // (every range has at least one stage)
-    const int part = t / tiles_mn;
-    kb0 = (int)((int64_t)p.nkb * part / p.ksplit);
-    kb1 = (int)((int64_t)p.nkb * (part + 1) / p.ksplit);
+  auto k_range = [&](int t, int &kb0, int &kb1) {      // (ranges of whole blocks of 128, none empty)
+    const int part = t / tiles_mn, blocks = (p.nkb + 1) / 2;
+    kb0 = 2 * (int)((int64_t)blocks * part / p.ksplit);
+    kb1 = 2 * (int)((int64_t)blocks * (part + 1) / p.ksplit);
+    kb1 = kb1 < p.nkb ? kb1 : p.nkb;
   };
   // groups of group_m row pairs, the column tiles of a group one after the other: the pairs that run at
   // the same time share a few bands of A and tiles of B in L2
@@ -244,11 +247,7 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
     const uint32_t row_addr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * 128);
     const uint32_t empty_leader[2] = {map_to_cta(acc_empty(0), 0), map_to_cta(acc_empty(1), 0)};
     float f0, f1;
-    unscale_factors(p.amax_a, p.amax_b, p.alpha_dev, p.alpha_exp, f0, f1);
-    // For logits one factor: where 2^-(e_a + e_b) leaves the range of fp32 it is held at the range's end (the
-    // logits are then below 2^-80, or beyond what their fp32 sum could hold)
-    const int e_ce = -((p.amax_a ? half_scale_exponent(*p.amax_a) : 0) + (p.amax_b ? half_scale_exponent(*p.amax_b) : 0));
-    const float f_ce = pow2f_exact(e_ce < -126 ? -126 : (e_ce > 126 ? 126 : e_ce)) * LOG2E;
+    alpha_factors(p.alpha_dev, p.alpha_exp, f0, f1);
     uint32_t j = 0;
     bool ok = true;
     for (int t = pair_id; t < num_items && ok; t += num_pairs) {
@@ -258,11 +257,19 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
       float acc[128];
 #pragma unroll
       for (int i = 0; i < 128; ++i) acc[i] = 0.f;
+      // the scale exponents along K of this CTA's block of A and this warp's block of B
+      const int64_t mblk = min(m0 >> 7, p.a_last), nblk = min((n0 + half * 128) >> 7, p.b_last);
+      const int *ea = p.ea ? p.ea + (A_MN ? mblk : mblk * p.ea_ld) : nullptr, *eb = p.eb ? p.eb + (B_MN ? nblk : nblk * p.eb_ld) : nullptr;
       for (int i = 0, n = kb1 - kb; i < n; ++i) {
         if (!f16_run_last<PROD, EPI>(i, n)) continue;
         const uint32_t b = j & 1;
+        const int64_t kblk = (kb + i) >> 1;
+        const int e = -((ea ? __ldg(ea + (A_MN ? kblk * p.ea_ld : kblk)) : 0) + (eb ? __ldg(eb + (B_MN ? kblk * p.eb_ld : kblk)) : 0));
         if (!mbar_wait(acc_full((int)b), (j >> 1) & 1, 55)) { ok = false; break; }
         tc_fence_after();
+        // the run's sum, unscaled, is added with one rounding (two factors where one leaves fp32's range)
+        const bool one = e >= -126 && e <= 127;
+        const float s0 = pow2f_exact(one ? e : e / 2), s1 = one ? 1.f : pow2f_exact(e - e / 2);
 #pragma unroll
         for (int c = 0; c < 4; c += 2) {
           uint32_t r0[32], r1[32];
@@ -274,10 +281,18 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
             __syncwarp();
             if (lane == 0) mbar_arrive_remote(empty_leader[b]);
           }
+          if (one) {
 #pragma unroll
-          for (int u = 0; u < 32; ++u) {
-            acc[32 * c + u] += __uint_as_float(r0[u]);
-            acc[32 * c + 32 + u] += __uint_as_float(r1[u]);
+            for (int u = 0; u < 32; ++u) {
+              acc[32 * c + u] = fmaf(__uint_as_float(r0[u]), s0, acc[32 * c + u]);
+              acc[32 * c + 32 + u] = fmaf(__uint_as_float(r1[u]), s0, acc[32 * c + 32 + u]);
+            }
+          } else {
+#pragma unroll
+            for (int u = 0; u < 32; ++u) {
+              acc[32 * c + u] = fmaf(__uint_as_float(r0[u]) * s0, s1, acc[32 * c + u]);
+              acc[32 * c + 32 + u] = fmaf(__uint_as_float(r1[u]) * s0, s1, acc[32 * c + 32 + u]);
+            }
           }
         }
         ++j;
@@ -346,18 +361,18 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
         // this lane's target among the warp's 128 columns, or -1
         const int tl = (tg >= (float)v0 && tg < (float)(v0 + 128)) ? (int)((int64_t)tg - v0) : -1;
         const bool any_target = __any_sync(0xffffffffu, tl >= 0);
-        // Logits are kept in units of log2 e (f_ce holds the factor), so that an exponential is one
-        // MUFU operation on a difference: a rounding of 2^-24 of the logit, as in any fp32 logit.
+        // Logits are kept in units of log2 e, so that an exponential is one MUFU operation on a difference: a
+        // rounding of 2^-24 of the logit, as in any fp32 logit.
         float bv[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) bv[c] = p.bias && nb + 32 * c + lane < p.N ? __ldg(p.bias + nb + 32 * c + lane) * LOG2E : 0.f;
         if constexpr (EPI == F16_STATS) {
           if (p.bias) {
 #pragma unroll
-            for (int i = 0; i < 128; ++i) acc[i] = fmaf(acc[i], f_ce, __shfl_sync(0xffffffffu, bv[i >> 5], i & 31));
+            for (int i = 0; i < 128; ++i) acc[i] = fmaf(acc[i], LOG2E, __shfl_sync(0xffffffffu, bv[i >> 5], i & 31));
           } else {
 #pragma unroll
-            for (int i = 0; i < 128; ++i) acc[i] *= f_ce;
+            for (int i = 0; i < 128; ++i) acc[i] *= LOG2E;
           }
           if (nb + 128 > p.N) {
 #pragma unroll
@@ -393,10 +408,10 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
             // p = 2^(l - lse), d = (p - [target]) coef
             if (p.bias) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = exp2_fast(fmaf(acc[32 * c + i], f_ce, __shfl_sync(0xffffffffu, bv[c], i) - lse));
+              for (int i = 0; i < 32; ++i) v[i] = exp2_fast(fmaf(acc[32 * c + i], LOG2E, __shfl_sync(0xffffffffu, bv[c], i) - lse));
             } else {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = exp2_fast(fmaf(acc[32 * c + i], f_ce, -lse));
+              for (int i = 0; i < 32; ++i) v[i] = exp2_fast(fmaf(acc[32 * c + i], LOG2E, -lse));
             }
             if (any_target) {
 #pragma unroll
@@ -452,12 +467,12 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
   }
 }
 
-// C = act(sum over the ranges of K, in order, unscaled, + bias), or C += it. Four consecutive columns per
+// C = act(alpha * sum over the ranges of K, in order, + bias), or C += it. Four consecutive columns per
 // thread (the rows of the work space are 16-byte aligned).
 __global__ void __launch_bounds__(256)
 gemm_f16_finish_kernel(const F16Params p, const float *__restrict__ partial, int64_t ld_partial, int64_t slice, int parts) {
   float f0, f1;
-  unscale_factors(p.amax_a, p.amax_b, p.alpha_dev, p.alpha_exp, f0, f1);
+  alpha_factors(p.alpha_dev, p.alpha_exp, f0, f1);
   const uint32_t per_row = (uint32_t)((p.N + 3) / 4);
   const int64_t total = (int64_t)p.M * per_row, step = (int64_t)gridDim.x * blockDim.x;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
@@ -526,103 +541,155 @@ int launch_column_sums(const float *part, int parts, int64_t N, float scale, con
 }
 
 // ---------------------------------------------------------------------------- passes over fp32 arrays
-// Eight consecutive columns per thread; vec: 128-bit loads (leading dimension and base allow them). CTAs
-// [0, split) work on the first array, the others on the second.
+// One CTA of 512 threads per block of 128 x 128: a warp takes 8 rows 16 apart, a lane four columns, so that the
+// block stays in registers between its maximum and its pair; every array is read once. With two CTAs per SM
+// 128 KB are in flight on each.
 struct HalfJobs {
-  HalfJob job[2];
-  bool vec[2];
-  int split;
+  HalfJob job[3];
+  bool vec[3], vec_out[3];     // 128-bit reads of x and of out
+  int begin[3];                // first CTA of each array
+  int n;
 };
-__device__ __forceinline__ void load8(const float *src, int64_t left, bool vec, float (&v)[8]) {
-  if (vec && left >= 8) {
-    const float4 a = __ldg(reinterpret_cast<const float4 *>(src)), b = __ldg(reinterpret_cast<const float4 *>(src) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+// Four values of a kept array, from column c (a multiple of 4).
+__device__ __forceinline__ void kept4(const Kept &k, int64_t r, int64_t c, float (&v)[4]) {
+  const uint32_t w = __ldg(reinterpret_cast<const uint32_t *>(k.q + r * k.ldq + c));
+  const float unit = pow2f_exact((int)__ldg(k.e + r * k.lde + (c >> 5)) - 127);
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int n = (int)(int8_t)((w >> (8 * u)) & 0xFFu);
+    v[u] = n == -128 ? NAN : (float)n * unit;
+  }
+}
+__device__ __forceinline__ void load4(const float *src, int64_t left, bool vec, float (&v)[4]) {
+  if (vec && left >= 4) {
+    const float4 a = __ldg(reinterpret_cast<const float4 *>(src));
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < left ? __ldg(src + i) : 0.f;
+    for (int i = 0; i < 4; ++i) v[i] = i < left ? __ldg(src + i) : 0.f;
   }
 }
-template <typename F>
-__device__ __forceinline__ void for_groups_of_8(const HalfJobs &jobs, F f) {
-  const bool second = (int)blockIdx.x >= jobs.split;
-  const HalfJob &j = jobs.job[second ? 1 : 0];
-  const bool vec = jobs.vec[second ? 1 : 0];
-  const int block = (int)blockIdx.x - (second ? jobs.split : 0), blocks = second ? (int)gridDim.x - jobs.split : jobs.split;
-  const int64_t per_row = (j.cols + 7) / 8, total = j.rows * per_row, step = (int64_t)blocks * blockDim.x;
-  const bool narrow = total < ((int64_t)1 << 31);
-  for (int64_t i = (int64_t)block * blockDim.x + threadIdx.x; i < total; i += step) {
-    const int64_t r = narrow ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row, c = (i - r * per_row) * 8;
-    f(j, vec, r, c);
-  }
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
+  return b < 0x7F800000u ? b : 0u;
 }
 
-__global__ void __launch_bounds__(256) amax_kernel(const __grid_constant__ HalfJobs jobs) {
+__global__ void __launch_bounds__(512, 2) half_split_kernel(const __grid_constant__ HalfJobs jobs) {
+  __shared__ uint32_t wmax[16];
+  __shared__ float part[16][HALF_BLOCK];
+  const int which = jobs.n > 2 && (int)blockIdx.x >= jobs.begin[2] ? 2 : (jobs.n > 1 && (int)blockIdx.x >= jobs.begin[1] ? 1 : 0);
+  const HalfJob &j = jobs.job[which];
+  const bool vec = jobs.vec[which], vec_out = jobs.vec_out[which];
+  const int block = (int)blockIdx.x - jobs.begin[which], bcols = (int)((j.cols + HALF_BLOCK - 1) / HALF_BLOCK);
+  const int rb = block / bcols, cb = block - rb * bcols;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t c = (int64_t)cb * HALF_BLOCK + 4 * lane, left = j.cols - c;
+  float v[8][4];
   uint32_t best = 0;
-  for_groups_of_8(jobs, [&](const HalfJob &j, bool vec, int64_t r, int64_t c) {
-    if (j.target && __ldg(j.target + r) < 0.f) return;
-    float v[8];
-    load8(j.x + r * j.ld + c, j.cols - c, vec, v);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const uint32_t b = __float_as_uint(v[k]) & 0x7FFFFFFFu;
-      if (b < 0x7F800000u && b > best) best = b;
+  for (int i = 0; i < 8; ++i) {
+    const int64_t r = (int64_t)rb * HALF_BLOCK + w + 16 * i;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[i][u] = 0.f;
+    if (r < j.rows && left > 0 && !(j.target && __ldg(j.target + r) < 0.f)) {
+      if (j.x) load4(j.x + r * j.ld + c, left, vec, v[i]);
+      else kept4(j.kept, r, c, v[i]);
+      if (j.act) {
+        float o[4];
+        if (j.out) load4(j.out + r * j.cols + c, left, vec_out, o);
+        else kept4(j.out_kept, r, c, o);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[i][u] = u < left ? v[i][u] * act_bwd(j.act, o[u]) : 0.f;
+      }
     }
-  });
-  best = __reduce_max_sync(0xffffffffu, best);
-  // (a maximum: any order gives the same bits)
-  if ((threadIdx.x & 31) == 0 && best) atomicMax(jobs.job[(int)blockIdx.x >= jobs.split ? 1 : 0].amax, best);
-}
-
-__global__ void __launch_bounds__(256) half_split_kernel(const __grid_constant__ HalfJobs jobs) {
-  const float s = half_scale(jobs.job[(int)blockIdx.x >= jobs.split ? 1 : 0].amax);
-  for_groups_of_8(jobs, [&](const HalfJob &j, bool vec, int64_t r, int64_t c) {
-    float v[8];
-    if (j.target && __ldg(j.target + r) < 0.f) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = 0.f;
-    } else {
-      load8(j.x + r * j.ld + c, j.cols - c, vec, v);
+    for (int u = 0; u < 4; ++u) best = max(best, finite_bits(v[i][u]));
+  }
+  if (j.keep.q) {
+    // the 8-bit form (keep8.cu): 8 lanes share a scale
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t r = (int64_t)rb * HALF_BLOCK + w + 16 * i;
+      uint32_t mx = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) mx = max(mx, finite_bits(v[i][u]));
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      // max / 2^e < 127.5: 127.5 = 64 * 1.9921875
+      int e = (int)(mx >> 23) - 127 - 6 + ((mx & 0x7FFFFFu) >= 0x7F0000u ? 1 : 0);
+      e = e < -126 ? -126 : (e > 121 ? 121 : e);
+      const float down = pow2f_exact(-e);
+      uint32_t q = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t b = __float_as_uint(v[i][u]) & 0x7FFFFFFFu;
+        int n = b < 0x7F800000u ? max(-127, min(127, __float2int_rn(v[i][u] * down))) : -128;
+        if (j.keep_sign && n == 0 && b != 0) n = v[i][u] < 0.f ? -1 : 1;
+        q |= ((uint32_t)n & 0xFFu) << (8 * u);
+      }
+      if (r < j.rows && c < j.keep.ldq) {
+        *reinterpret_cast<uint32_t *>(j.keep.q + r * j.keep.ldq + c) = q;
+        if ((lane & 7) == 0) j.keep.e[r * j.keep.lde + (c >> 5)] = (uint8_t)(e + 127);
+      }
     }
-    __half h[8], l[8];
+  }
+  if (j.hi) {
+    best = __reduce_max_sync(0xffffffffu, best);
+    if (lane == 0) wmax[w] = best;
+    __syncthreads();
+    best = __reduce_max_sync(0xffffffffu, wmax[lane & 15]);
+    const int ex = half_scale_exponent(best);
+    if (threadIdx.x == 0) j.e[block] = ex;
+    const float s = pow2f_exact(ex);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) half_pair(v[k] * s, h[k], l[k]);
-    // (ld_out covers whole groups of 8)
-    *reinterpret_cast<uint4 *>(j.hi + r * j.ld_out + c) = *reinterpret_cast<uint4 *>(h);
-    *reinterpret_cast<uint4 *>(j.lo + r * j.ld_out + c) = *reinterpret_cast<uint4 *>(l);
-  });
+    for (int i = 0; i < 8; ++i) {
+      const int64_t r = (int64_t)rb * HALF_BLOCK + w + 16 * i;
+      if (r < j.rows && left > 0) {        // (ld_out covers whole groups of 4)
+        __half h[4], l[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) half_pair(v[i][u] * s, h[u], l[u]);
+        *reinterpret_cast<uint2 *>(j.hi + r * j.ld_out + c) = *reinterpret_cast<uint2 *>(h);
+        if (j.lo) *reinterpret_cast<uint2 *>(j.lo + r * j.ld_out + c) = *reinterpret_cast<uint2 *>(l);
+      }
+    }
+  }
+  if (j.sums) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      float t = v[0][u];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) t += v[i][u];
+      part[w][4 * lane + u] = t;
+    }
+    __syncthreads();
+    if (threadIdx.x < HALF_BLOCK) {
+      float t = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) t += part[i][threadIdx.x];
+      const int64_t n = (int64_t)cb * HALF_BLOCK + threadIdx.x;
+      if (n < j.cols) j.sums[rb * j.cols + n] = t;
+    }
+  }
 }
 
 static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Splits the grid of a pass by the arrays' sizes; 0 CTAs when there is nothing to do.
-static int plan_jobs(HalfJobs &jobs, const HalfJob &a, const HalfJob *b, bool flat) {
-  int64_t groups[2] = {0, 0};
-  for (int i = 0; i < 2; ++i) {
-    if (i == 1 && !b) break;
-    HalfJob &j = jobs.job[i] = i == 0 ? a : *b;
-    if (flat && !j.target && j.ld == j.cols) { j.cols *= j.rows; j.ld = j.cols; j.rows = j.cols > 0 ? 1 : 0; }
-    jobs.vec[i] = aligned16(j.x) && (j.ld % 4 == 0 || j.rows == 1);
-    groups[i] = j.rows * ceil_div(j.cols, 8);
+int launch_half_split(const HalfJob *jobs, int n, cudaStream_t s) {
+  HalfJobs a;
+  int64_t grid = 0;
+  a.n = 0;
+  for (int i = 0; i < n; ++i) {
+    if (jobs[i].rows <= 0 || jobs[i].cols <= 0) continue;
+    a.job[a.n] = jobs[i];
+    a.vec[a.n] = aligned16(jobs[i].x) && (jobs[i].ld % 4 == 0 || jobs[i].rows == 1);
+    a.vec_out[a.n] = aligned16(jobs[i].out) && jobs[i].cols % 4 == 0;
+    a.begin[a.n] = (int)grid;
+    grid += half_blocks(jobs[i].rows) * half_blocks(jobs[i].cols);
+    ++a.n;
   }
-  const int g0 = groups[0] ? grid_for(groups[0], 256, 8) : 0, g1 = groups[1] ? grid_for(groups[1], 256, 8) : 0;
-  jobs.split = g0;
-  return g0 + g1;
-}
-
-int launch_amax(const HalfJob &a, const HalfJob *b, cudaStream_t s) {
-  HalfJobs jobs;
-  const int grid = plan_jobs(jobs, a, b, true);
   if (grid == 0) return ENDIA_B200_OK;
-  amax_kernel<<<grid, 256, 0, s>>>(jobs);
-  EB_LAUNCH_CHECK();
-  return ENDIA_B200_OK;
-}
-
-int launch_half_split(const HalfJob &a, const HalfJob *b, cudaStream_t s) {
-  HalfJobs jobs;
-  const int grid = plan_jobs(jobs, a, b, false);
-  if (grid == 0) return ENDIA_B200_OK;
-  half_split_kernel<<<grid, 256, 0, s>>>(jobs);
+  EB_REQUIRE(grid < ((int64_t)1 << 31), ENDIA_B200_ELIMIT, "fp16-pair product: operands of more than 2^45 elements");
+  half_split_kernel<<<(unsigned)grid, 512, 0, s>>>(a);
   EB_LAUNCH_CHECK();
   return ENDIA_B200_OK;
 }
@@ -718,7 +785,9 @@ int launch_gemm_f16(const F16Gemm &g, bool a_mn, bool b_mn, int epilogue, cudaSt
   p.group_m = 8;
   p.nkb = (int)ceil_div(g.K, F16_BK);
   p.ksplit = 1;
-  p.amax_a = g.a.amax; p.amax_b = g.b.amax; p.alpha_dev = g.alpha_dev; p.alpha_exp = g.alpha_exp; p.bias = g.bias;
+  p.ea = g.a.e; p.ea_ld = g.a.e_ld; p.a_last = (int)half_blocks(g.M) - 1;
+  p.eb = g.b.e; p.eb_ld = g.b.e_ld; p.b_last = (int)half_blocks(g.N) - 1;
+  p.alpha_dev = g.alpha_dev; p.alpha_exp = g.alpha_exp; p.bias = g.bias;
   p.C = g.C; p.ldc = g.ldc; p.act = g.act; p.accumulate = g.accumulate ? 1 : 0;
   p.target = g.target; p.n_base = g.n_base; p.stats = g.stats; p.target_logit = g.target_logit;
   p.lse = g.lse; p.coef = g.coef; p.colsum_part = g.colsum_part;

@@ -1,21 +1,26 @@
 // fp32-accurate matrix products from fp16 pairs on the tensor cores (gemm_f16.cu), the engine of the
 // cross entropy over a large vocabulary and of the layers checkpointed in 8 bits.
-//   x * s = hi + lo,  hi = fp16(x * s), lo = fp16(x * s - hi),  s a power of two from the largest
-//   finite |x| of the operand so that it lands in [2^14, 2^15)
-// hi and lo hold 22 bits of every element down to 2^-15 of the largest one; smaller ones are exact to
-// 2^-40 of it.  a*b = a_hi*b_hi + a_lo*b_hi + a_hi*b_lo (+ a_lo*b_lo, 2^-24 of the product, dropped).
+//   x * s = hi + lo,  hi = fp16(x * s), lo = fp16(x * s - hi),  s a power of two per block of 128 x 128
+//   elements that puts the block's largest finite |x| into [2^14, 2^15)
+// hi and lo hold 22 bits of every element down to 2^-15 of the largest one of its block; smaller ones are
+// exact to 2^-40 of it.  a*b = a_hi*b_hi + a_lo*b_hi + a_hi*b_lo (+ a_lo*b_lo, 2^-24 of the product, dropped).
+// The blocks' scales come out again where the accumulators are added in fp32: a run of 64 or 128 of K lies in one
+// block of each operand. A scale per array would need the array's maximum first, one more pass over it.
 #pragma once
 #include "common.cuh"
 #include <cuda_fp16.h>
 
 namespace eb {
 
+constexpr int HALF_BLOCK = 128;
+
 // An operand laid out row-major with leading dimension ld (a multiple of 8), 16-byte aligned.
 struct HalfPair {
   const __half *hi = nullptr;
   const __half *lo = nullptr;       // NULL: the operand is exact in hi
   int64_t ld = 0;
-  const uint32_t *amax = nullptr;   // device: bits of the largest finite |x| (the scale s follows from it); NULL: s = 1
+  const int *e = nullptr;           // scale exponents [row blocks][e_ld] (s = 2^e); NULL: 1
+  int64_t e_ld = 0;
 };
 
 enum F16Epilogue {
@@ -29,7 +34,7 @@ constexpr float F16_D_SCALE = 32768.f;      // 2^F16_D_EXP
 struct F16Gemm {
   int64_t M = 0, N = 0, K = 0;
   HalfPair a, b;
-  const float *alpha_dev = nullptr;   // optional device scalar multiplied into v, and 2^alpha_exp
+  const float *alpha_dev = nullptr;   // F16_STORE: optional device scalar multiplied into v, and 2^alpha_exp
   int alpha_exp = 0;
   const float *bias = nullptr;        // [N]
   // F16_STORE
@@ -55,20 +60,41 @@ int launch_gemm_f16(const F16Gemm &g, bool a_mn, bool b_mn, int epilogue, cudaSt
 size_t gemm_f16_partial_bytes(int64_t M, int64_t N, int64_t K);
 bool gemm_f16_available();
 
-// One fp32 array of the passes below: [rows, cols], leading dimension ld. `target` (optional, [rows]):
-// rows with target < 0 do not count in the maximum and become zero in the pair.
-struct HalfJob {
-  const float *x = nullptr;
-  int64_t rows = 0, cols = 0, ld = 0;
-  const float *target = nullptr;
-  uint32_t *amax = nullptr;      // bits of the largest finite |x|
-  __half *hi = nullptr, *lo = nullptr;
-  int64_t ld_out = 0;
+// The 8-bit form of an activation (keep8.cu): q [rows][cols rounded up to 32], then e + 127 [rows][ldq / 32].
+struct Kept {
+  int8_t *q = nullptr;
+  uint8_t *e = nullptr;
+  int64_t ldq = 0, lde = 0;
 };
-// amax[0] = max(amax[0], bits of the largest finite |x|) of up to two arrays in one launch; *amax starts at 0.
-int launch_amax(const HalfJob &a, const HalfJob *b, cudaStream_t s);
-// The fp16 pairs of up to two arrays in one launch.
-int launch_half_split(const HalfJob &a, const HalfJob *b, cudaStream_t s);
+__host__ __device__ inline Kept kept_view(void *p, int64_t rows, int64_t cols) {
+  Kept k;
+  k.ldq = (cols + 31) / 32 * 32;
+  k.lde = k.ldq / 32;
+  k.q = static_cast<int8_t *>(p);
+  k.e = static_cast<uint8_t *>(p) + rows * k.ldq;
+  return k;
+}
+
+// One array of the pass that makes operands: read once, block by block.
+struct HalfJob {
+  int64_t rows = 0, cols = 0;
+  const float *x = nullptr;          // [rows][ld], or NULL: `kept`
+  int64_t ld = 0;
+  Kept kept;
+  const float *target = nullptr;     // [rows], optional: rows with target < 0 read as zero
+  int act = 0;                       // != 0: x times act'(out), out contiguous fp32, or NULL: `out_kept`
+  const float *out = nullptr;
+  Kept out_kept;
+  __half *hi = nullptr, *lo = nullptr;   // the pair (hi NULL: none; lo NULL: exact in hi)
+  int64_t ld_out = 0;
+  int *e = nullptr;                  // the blocks' scale exponents, [ceil(rows / 128)][ceil(cols / 128)]
+  Kept keep;                         // q != NULL: the 8-bit form is written too
+  int keep_sign = 0;
+  float *sums = nullptr;             // optional: [ceil(rows / 128)][cols] sums over 128 rows
+};
+inline int64_t half_blocks(int64_t n) { return ceil_div(n, HALF_BLOCK); }
+// Up to three arrays in one launch.
+int launch_half_split(const HalfJob *jobs, int n, cudaStream_t s);
 
 // out[n] = the sum of the rows of part [parts][N], in a fixed order, times scale, times alpha (a device scalar, NULL: 1).
 int launch_column_sums(const float *part, int parts, int64_t N, float scale, const float *alpha, float *out, cudaStream_t s);
@@ -83,22 +109,19 @@ struct Carver {       // a caller's work space, handed out in 256-byte steps (ba
   }
 };
 
-// Scale of an operand from its largest finite |x|: 2^(14 - floor(log2 amax)), at most 2^126 (an operand of
-// values below 2^-112 keeps fewer than 22 bits, down to those of a denormal), and its inverse.
+// Scale exponent of a block from its largest finite |x|: 14 - floor(log2 amax), at most 126 (a block of
+// values below 2^-112 keeps fewer than 22 bits, down to those of a denormal).
 __host__ __device__ __forceinline__ int half_scale_exponent(uint32_t amax_bits) {
   if (amax_bits == 0) return 0;
   const int ex = 141 - (int)(amax_bits >> 23);
   return ex > 126 ? 126 : ex;
 }
 __device__ __forceinline__ float pow2f_exact(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }   // -126 <= e <= 127
-__device__ __forceinline__ float half_scale(const uint32_t *amax) { return amax ? pow2f_exact(half_scale_exponent(*amax)) : 1.f; }
 
-// A sum of scaled products is (sum * f0) * f1: the operands' unscaling, `alpha` (optional device scalar) and
-// 2^extra as two factors of about the same exponent, so that neither step leaves the range of fp32 unless
-// the result does.
-__device__ __forceinline__ void unscale_factors(const uint32_t *amax_a, const uint32_t *amax_b, const float *alpha, int extra,
-                                                float &f0, float &f1) {
-  int e = extra - (amax_a ? half_scale_exponent(*amax_a) : 0) - (amax_b ? half_scale_exponent(*amax_b) : 0);
+// alpha (optional device scalar) times 2^extra as two factors of about the same exponent, so that (v * f0) * f1
+// leaves the range of fp32 only where the result does.
+__device__ __forceinline__ void alpha_factors(const float *alpha, int extra, float &f0, float &f1) {
+  int e = extra;
   float m = 1.f;
   if (alpha) {
     m = *alpha;
@@ -109,8 +132,8 @@ __device__ __forceinline__ void unscale_factors(const uint32_t *amax_a, const ui
     }
   }
   const int e0 = e / 2, e1 = e - e0;
-  f0 = m * pow2f_exact(e0 < -126 ? -126 : (e0 > 126 ? 126 : e0));
-  f1 = pow2f_exact(e1 < -126 ? -126 : (e1 > 127 ? 127 : e1));
+  f0 = m * pow2f_exact(e0);
+  f1 = pow2f_exact(e1);
 }
 
 // hi and lo of a scaled value. An infinite or NaN value gives an infinite or NaN hi and a NaN lo.

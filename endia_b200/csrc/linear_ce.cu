@@ -18,8 +18,7 @@ using namespace eb;
 
 namespace eb {
 
-// state: [0] rows that count, [1] and [2] the scales' maxima of x and W (bits), [3] CTAs of ce_rows_kernel
-// that are done, [4 ...) lse per row, then lse log2 e per row. Inside, logits are in units of log2 e: exponentials are powers of two.
+// state: [0] rows that count, [1] CTAs of ce_rows_kernel that are done, [4 ...) lse per row, then lse log2 e per row. Inside, logits are in units of log2 e: exponentials are powers of two.
 constexpr double CE_LOG2E = 1.4426950408889634, CE_LN2 = 0.6931471805599453;
 constexpr int CE_STATE_HEAD = 4;
 // Work space for one piece of the vocabulary (the d pair and W's pair, 4 bytes each per element).
@@ -69,7 +68,7 @@ ce_rows_kernel(const float2 *__restrict__ stats, int parts, const float *__restr
     __threadfence();
   }
   __syncthreads();
-  if (threadIdx.x == 0) last = atomicAdd(reinterpret_cast<unsigned int *>(state) + 3, 1u) == gridDim.x - 1;
+  if (threadIdx.x == 0) last = atomicAdd(reinterpret_cast<unsigned int *>(state) + 1, 1u) == gridDim.x - 1;
   __syncthreads();
   if (!last) return;
   float s = 0.f;
@@ -250,7 +249,7 @@ static int64_t ce_piece(int64_t bytes_per_column, int64_t V) {
   return ceil_div(ceil_div(V, pieces), 256) * 256;
 }
 
-struct CeForward { float2 *stats; float *tl, *rows; __half *xh, *xl, *wh, *wl; int64_t piece, parts, ldx; };
+struct CeForward { float2 *stats; float *tl, *rows; __half *xh, *xl, *wh, *wl; int *xe, *we; int64_t piece, parts, ldx; };
 static size_t ce_carve_forward(int64_t M, int64_t K, int64_t V, char *base, CeForward &f) {
   Carver c{base};
   f = CeForward{};
@@ -264,22 +263,25 @@ static size_t ce_carve_forward(int64_t M, int64_t K, int64_t V, char *base, CeFo
     f.ldx = ceil_div(K, 8) * 8;
     f.xh = c.take<__half>(M * f.ldx); f.xl = c.take<__half>(M * f.ldx);
     f.wh = c.take<__half>(K * f.piece); f.wl = c.take<__half>(K * f.piece);
+    f.xe = c.take<int>(half_blocks(M) * half_blocks(K));
+    f.we = c.take<int>(half_blocks(K) * half_blocks(f.piece));
   }
   f.stats = c.take<float2>(M * f.parts);
   return c.used;
 }
 
-struct CeBackward { float *coef, *alpha, *partial, *part_sums; uint32_t *amax; __half *xh, *xl, *wh, *wl, *dh, *dl; int64_t piece, ldx; };
+struct CeBackward { float *coef, *alpha, *partial, *part_sums; __half *xh, *xl, *wh, *wl, *dh, *dl; int *xe, *we; int64_t piece, ldx; };
 static size_t ce_carve_backward(int64_t M, int64_t K, int64_t V, char *base, CeBackward &f) {
   Carver c{base};
   f = CeBackward{};
   f.coef = c.take<float>(M);
   f.alpha = c.take<float>(1);
-  f.amax = c.take<uint32_t>(2);
   f.piece = ce_piece(4 * (M + K), V);
   f.ldx = ceil_div(K, 8) * 8;
   f.xh = c.take<__half>(M * f.ldx); f.xl = c.take<__half>(M * f.ldx);
   f.wh = c.take<__half>(K * f.piece); f.wl = c.take<__half>(K * f.piece);
+  f.xe = c.take<int>(half_blocks(M) * half_blocks(K));
+  f.we = c.take<int>(half_blocks(K) * half_blocks(f.piece));
   f.dh = c.take<__half>(M * f.piece); f.dl = c.take<__half>(M * f.piece);
   f.part_sums = c.take<float>(ceil_div(M, 32) * f.piece);
   size_t a = gemm_f16_partial_bytes(M, K, f.piece), b = gemm_f16_partial_bytes(K, f.piece, M);
@@ -288,6 +290,15 @@ static size_t ce_carve_backward(int64_t M, int64_t K, int64_t V, char *base, CeB
   a = a > a2 ? a : a2; b = b > b2 ? b : b2;
   f.partial = reinterpret_cast<float *>(c.take<char>((int64_t)(a > b ? a : b)));
   return c.used;
+}
+
+// The passes over a piece of W (the caller sets its columns) and, with the first one, over x.
+template <typename F>
+static void ce_jobs(HalfJob (&jobs)[2], const float *x, int64_t ldx, const float *W, int64_t ldw, const float *target, int64_t M,
+                    int64_t K, const F &f) {
+  HalfJob &jw = jobs[0], &jx = jobs[1];
+  jw.rows = K; jw.x = W; jw.ld = ldw; jw.hi = f.wh; jw.lo = f.wl; jw.ld_out = f.piece; jw.e = f.we;
+  jx.rows = M; jx.cols = K; jx.x = x; jx.ld = ldx; jx.target = target; jx.hi = f.xh; jx.lo = f.xl; jx.ld_out = f.ldx; jx.e = f.xe;
 }
 
 static int ce_check(const float *x, int64_t ldx, const float *W, int64_t ldw, const float *target, int64_t M, int64_t K,
@@ -334,23 +345,21 @@ int endia_b200_linear_ce_fwd(const float *x, int64_t ldx, const float *W, int64_
   CeForward f;
   ce_carve_forward(M, K, V, static_cast<char *>(scratch), f);
   float *rows = reduction == ENDIA_B200_LOSS_NONE ? loss : f.rows;
-  uint32_t *amax = reinterpret_cast<uint32_t *>(state) + 1;
   if (ce_few_rows(M)) {
     const auto few = M <= 1 ? launch_few_rows<1> : M <= 2 ? launch_few_rows<2> : M <= 4 ? launch_few_rows<4>
                      : M <= 8 ? launch_few_rows<8> : launch_few_rows<CE_FEW>;
     if ((st = few(x, ldx, W, ldw, bias, target, (int)M, (int)K, (int)V, f.stats, f.tl, s))) return st;
   } else {
-    const HalfJob jx{x, M, K, ldx, target, amax, f.xh, f.xl, f.ldx};
-    HalfJob jw{W, K, V, ldw, nullptr, amax + 1, f.wh, f.wl, f.piece};
-    if ((st = launch_amax(jw, &jx, s))) return st;
+    HalfJob jobs[2];
+    ce_jobs(jobs, x, ldx, W, ldw, target, M, K, f);
     for (int64_t v0 = 0; v0 < V; v0 += f.piece) {
       const int64_t n = V - v0 < f.piece ? V - v0 : f.piece;
-      jw.x = W + v0; jw.cols = n;
-      if ((st = launch_half_split(jw, v0 ? nullptr : &jx, s))) return st;
+      jobs[0].x = W + v0; jobs[0].cols = n;
+      if ((st = launch_half_split(jobs, v0 ? 1 : 2, s))) return st;
       F16Gemm g;
       g.M = M; g.N = n; g.K = K;
-      g.a = HalfPair{f.xh, f.xl, f.ldx, amax};
-      g.b = HalfPair{f.wh, f.wl, f.piece, amax + 1};
+      g.a = HalfPair{f.xh, f.xl, f.ldx, f.xe, half_blocks(K)};
+      g.b = HalfPair{f.wh, f.wl, f.piece, f.we, half_blocks(n)};
       g.bias = bias ? bias + v0 : nullptr;
       g.target = target; g.n_base = v0; g.stats = f.stats; g.target_logit = f.tl;
       if ((st = launch_gemm_f16(g, false, true, F16_STATS, s))) return st;
@@ -380,36 +389,30 @@ int endia_b200_linear_ce_bwd(const float *x, int64_t ldx, const float *W, int64_
   CeBackward f;
   ce_carve_backward(M, K, V, static_cast<char *>(scratch), f);
   const float *lse = state + CE_STATE_HEAD + M;      // (in units of log2 e)
-  uint32_t *amax = const_cast<uint32_t *>(reinterpret_cast<const uint32_t *>(state)) + 1;      // (read only)
   ce_coef_kernel<<<1, 1024, 0, s>>>(grad, reduction == ENDIA_B200_LOSS_NONE, reduction == ENDIA_B200_LOSS_MEAN, state, target,
                                     (int)M, (int)V, f.coef, f.alpha);
   EB_LAUNCH_CHECK();
-  HalfJob jx{x, M, K, ldx, target, amax, f.xh, f.xl, f.ldx}, jw{W, K, V, ldw, nullptr, amax + 1, f.wh, f.wl, f.piece};
-  if (ce_few_rows(M)) {      // the forward pass ran in fp32 and left no scales
-    jx.amax = amax = f.amax;
-    jw.amax = amax + 1;
-    EB_CUDA(cudaMemsetAsync(f.amax, 0, 2 * sizeof(uint32_t), s));
-    if ((st = launch_amax(jw, &jx, s))) return st;
-  }
+  HalfJob jobs[2];
+  ce_jobs(jobs, x, ldx, W, ldw, target, M, K, f);
   for (int64_t v0 = 0; v0 < V; v0 += f.piece) {
     const int64_t n = V - v0 < f.piece ? V - v0 : f.piece;
-    jw.x = W + v0; jw.cols = n;
-    if ((st = launch_half_split(jw, v0 ? nullptr : &jx, s))) return st;
+    jobs[0].x = W + v0; jobs[0].cols = n;
+    if ((st = launch_half_split(jobs, v0 ? 1 : 2, s))) return st;
     F16Gemm g;
     g.M = M; g.N = n; g.K = K;
-    g.a = HalfPair{f.xh, f.xl, f.ldx, amax};
-    g.b = HalfPair{f.wh, f.wl, f.piece, amax + 1};
+    g.a = HalfPair{f.xh, f.xl, f.ldx, f.xe, half_blocks(K)};
+    g.b = HalfPair{f.wh, f.wl, f.piece, f.we, half_blocks(n)};
     g.bias = bias ? bias + v0 : nullptr;
     g.target = target; g.n_base = v0; g.lse = lse; g.coef = f.coef;
     g.d_hi = f.dh; g.d_lo = f.dl; g.ld_d = f.piece;
     g.colsum_part = db ? f.part_sums : nullptr;
     if ((st = launch_gemm_f16(g, false, true, F16_DLOGITS, s))) return st;
-    const HalfPair d{f.dh, f.dl, f.piece, nullptr};
+    const HalfPair d{f.dh, f.dl, f.piece, nullptr, 0};
     if (dx) {      // dx += d W^T, over the pieces in order
       F16Gemm h;
       h.M = M; h.N = K; h.K = n;
       h.a = d;
-      h.b = HalfPair{f.wh, f.wl, f.piece, amax + 1};
+      h.b = HalfPair{f.wh, f.wl, f.piece, f.we, half_blocks(n)};
       h.alpha_dev = f.alpha; h.alpha_exp = -F16_D_EXP;
       h.C = dx; h.ldc = K; h.accumulate = v0 > 0; h.partial = f.partial;
       if ((st = launch_gemm_f16(h, false, false, F16_STORE, s))) return st;
@@ -417,7 +420,7 @@ int endia_b200_linear_ce_bwd(const float *x, int64_t ldx, const float *W, int64_
     if (dw) {
       F16Gemm h;
       h.M = K; h.N = n; h.K = M;
-      h.a = HalfPair{f.xh, f.xl, f.ldx, amax};
+      h.a = HalfPair{f.xh, f.xl, f.ldx, f.xe, half_blocks(K)};
       h.b = d;
       h.alpha_dev = f.alpha; h.alpha_exp = -F16_D_EXP;
       h.C = dw + v0; h.ldc = V; h.partial = f.partial;

@@ -80,7 +80,7 @@ def test_error_bound_and_size(nd):
     got = read_back(nd, x, False)
     top = np.abs(x).reshape(256, 16, 32).max(2, keepdims=True)
     assert (np.abs(got - x).reshape(256, 16, 32) <= top / 63.75 / 2).all()
-    assert nd._lib.lib.endia_b200_keep8_bytes(256, 512) == 256 + 256 * 512 * 33 // 32
+    assert nd._lib.lib.endia_b200_keep8_bytes(256, 512) == 256 * 512 * 33 // 32
 
 
 def test_keep8_releases_and_reads_back(nd):
