@@ -246,8 +246,6 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
     const uint32_t ebuf = epi_base + (uint32_t)(warp - 4) * 4096u;
     const uint32_t row_addr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * 128);
     const uint32_t empty_leader[2] = {map_to_cta(acc_empty(0), 0), map_to_cta(acc_empty(1), 0)};
-    float f0, f1;
-    alpha_factors(p.alpha_dev, p.alpha_exp, f0, f1);
     uint32_t j = 0;
     bool ok = true;
     for (int t = pair_id; t < num_items && ok; t += num_pairs) {
@@ -260,16 +258,20 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
       // the scale exponents along K of this CTA's block of A and this warp's block of B
       const int64_t mblk = min(m0 >> 7, p.a_last), nblk = min((n0 + half * 128) >> 7, p.b_last);
       const int *ea = p.ea ? p.ea + (A_MN ? mblk : mblk * p.ea_ld) : nullptr, *eb = p.eb ? p.eb + (B_MN ? nblk : nblk * p.eb_ld) : nullptr;
+      auto unscale_of = [&](int kblk) {
+        return -((ea ? __ldg(ea + (A_MN ? kblk * p.ea_ld : kblk)) : 0) + (eb ? __ldg(eb + (B_MN ? kblk * p.eb_ld : kblk)) : 0));
+      };
+      // the tile's unit: the largest unscaling exponent along K
+      int unit = -1000;
+      for (int k = (kb >> 1) + lane; 2 * k < kb1; k += 32) unit = max(unit, unscale_of(k));
+      unit = __reduce_max_sync(0xffffffffu, unit);
       for (int i = 0, n = kb1 - kb; i < n; ++i) {
         if (!f16_run_last<PROD, EPI>(i, n)) continue;
         const uint32_t b = j & 1;
-        const int64_t kblk = (kb + i) >> 1;
-        const int e = -((ea ? __ldg(ea + (A_MN ? kblk * p.ea_ld : kblk)) : 0) + (eb ? __ldg(eb + (B_MN ? kblk * p.eb_ld : kblk)) : 0));
+        const int e = unscale_of((kb + i) >> 1) - unit;      // <= 0
         if (!mbar_wait(acc_full((int)b), (j >> 1) & 1, 55)) { ok = false; break; }
         tc_fence_after();
-        // the run's sum, unscaled, is added with one rounding (two factors where one leaves fp32's range)
-        const bool one = e >= -126 && e <= 127;
-        const float s0 = pow2f_exact(one ? e : e / 2), s1 = one ? 1.f : pow2f_exact(e - e / 2);
+        const float s0 = e < -126 ? 0.f : pow2f_exact(e);
 #pragma unroll
         for (int c = 0; c < 4; c += 2) {
           uint32_t r0[32], r1[32];
@@ -281,18 +283,10 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
             __syncwarp();
             if (lane == 0) mbar_arrive_remote(empty_leader[b]);
           }
-          if (one) {
 #pragma unroll
-            for (int u = 0; u < 32; ++u) {
-              acc[32 * c + u] = fmaf(__uint_as_float(r0[u]), s0, acc[32 * c + u]);
-              acc[32 * c + 32 + u] = fmaf(__uint_as_float(r1[u]), s0, acc[32 * c + 32 + u]);
-            }
-          } else {
-#pragma unroll
-            for (int u = 0; u < 32; ++u) {
-              acc[32 * c + u] = fmaf(__uint_as_float(r0[u]) * s0, s1, acc[32 * c + u]);
-              acc[32 * c + 32 + u] = fmaf(__uint_as_float(r1[u]) * s0, s1, acc[32 * c + 32 + u]);
-            }
+          for (int u = 0; u < 32; ++u) {
+            acc[32 * c + u] = fmaf(__uint_as_float(r0[u]), s0, acc[32 * c + u]);
+            acc[32 * c + 32 + u] = fmaf(__uint_as_float(r1[u]), s0, acc[32 * c + 32 + u]);
           }
         }
         ++j;
@@ -303,6 +297,8 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
 
       if constexpr (EPI == F16_STORE) {
         const bool parts = p.part_rows > 0;
+        float f0, f1;      // (the parts' alpha comes with their sum)
+        alpha_factors(parts ? nullptr : p.alpha_dev, unit + (parts ? 0 : p.alpha_exp), f0, f1);
         const int row_off = parts ? (t / tiles_mn) * p.part_rows : 0;
         const bool bulk = parts || p.vec_c;
 #pragma unroll
@@ -317,9 +313,7 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
               float4 v = make_float4(acc[32 * c + 4 * u], acc[32 * c + 4 * u + 1], acc[32 * c + 4 * u + 2], acc[32 * c + 4 * u + 3]);
-              if (!parts) {
-                v.x = (v.x * f0) * f1; v.y = (v.y * f0) * f1; v.z = (v.z * f0) * f1; v.w = (v.w * f0) * f1;
-              }
+              v.x = (v.x * f0) * f1; v.y = (v.y * f0) * f1; v.z = (v.z * f0) * f1; v.w = (v.w * f0) * f1;
               sts128(ebuf + (uint32_t)lane * 128u + (uint32_t)((u ^ (lane & 7)) * 16), v);
             }
             __syncwarp();
@@ -361,18 +355,20 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
         // this lane's target among the warp's 128 columns, or -1
         const int tl = (tg >= (float)v0 && tg < (float)(v0 + 128)) ? (int)((int64_t)tg - v0) : -1;
         const bool any_target = __any_sync(0xffffffffu, tl >= 0);
-        // Logits are kept in units of log2 e, so that an exponential is one MUFU operation on a difference: a
-        // rounding of 2^-24 of the logit, as in any fp32 logit.
+        // Logits in units of log2 e, so that an exponential is one MUFU operation on a difference: a rounding of
+        // 2^-24 of the logit, as in any fp32 logit. (One factor: a unit beyond its range belongs to logits below
+        // 2^-80, or to sums that fp32 does not hold.)
+        const float to_log2 = pow2f_exact(max(-126, min(126, unit))) * LOG2E;
         float bv[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) bv[c] = p.bias && nb + 32 * c + lane < p.N ? __ldg(p.bias + nb + 32 * c + lane) * LOG2E : 0.f;
         if constexpr (EPI == F16_STATS) {
           if (p.bias) {
 #pragma unroll
-            for (int i = 0; i < 128; ++i) acc[i] = fmaf(acc[i], LOG2E, __shfl_sync(0xffffffffu, bv[i >> 5], i & 31));
+            for (int i = 0; i < 128; ++i) acc[i] = fmaf(acc[i], to_log2, __shfl_sync(0xffffffffu, bv[i >> 5], i & 31));
           } else {
 #pragma unroll
-            for (int i = 0; i < 128; ++i) acc[i] *= LOG2E;
+            for (int i = 0; i < 128; ++i) acc[i] *= to_log2;
           }
           if (nb + 128 > p.N) {
 #pragma unroll
@@ -408,10 +404,10 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
             // p = 2^(l - lse), d = (p - [target]) coef
             if (p.bias) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = exp2_fast(fmaf(acc[32 * c + i], LOG2E, __shfl_sync(0xffffffffu, bv[c], i) - lse));
+              for (int i = 0; i < 32; ++i) v[i] = exp2_fast(fmaf(acc[32 * c + i], to_log2, __shfl_sync(0xffffffffu, bv[c], i) - lse));
             } else {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = exp2_fast(fmaf(acc[32 * c + i], LOG2E, -lse));
+              for (int i = 0; i < 32; ++i) v[i] = exp2_fast(fmaf(acc[32 * c + i], to_log2, -lse));
             }
             if (any_target) {
 #pragma unroll
@@ -574,6 +570,8 @@ __device__ __forceinline__ uint32_t finite_bits(float v) {
   return b < 0x7F800000u ? b : 0u;
 }
 
+// PLAIN: pairs of fp32 arrays and nothing else (fewer registers).
+template <bool PLAIN>
 __global__ void __launch_bounds__(512, 2) half_split_kernel(const __grid_constant__ HalfJobs jobs) {
   __shared__ uint32_t wmax[16];
   __shared__ float part[16][HALF_BLOCK];
@@ -584,32 +582,52 @@ __global__ void __launch_bounds__(512, 2) half_split_kernel(const __grid_constan
   const int rb = block / bcols, cb = block - rb * bcols;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t c = (int64_t)cb * HALF_BLOCK + 4 * lane, left = j.cols - c;
+  const int64_t row0 = (int64_t)rb * HALF_BLOCK + w;      // this warp's rows: row0 + 16 i
+  bool live[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) live[i] = row0 + 16 * i < j.rows && left > 0 && !(j.target && __ldg(j.target + row0 + 16 * i) < 0.f);
   float v[8][4];
-  uint32_t best = 0;
+  // (the eight loads are issued together: nothing uses one of them before the last is on its way)
+  if (!PLAIN && !j.x) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t r = (int64_t)rb * HALF_BLOCK + w + 16 * i;
+    for (int i = 0; i < 8; ++i) {
+      if (live[i]) kept4(j.kept, row0 + 16 * i, c, v[i]);
+      else v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
+    }
+  } else if (vec && (cb + 1) * HALF_BLOCK <= j.cols) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) v[i][u] = 0.f;
-    if (r < j.rows && left > 0 && !(j.target && __ldg(j.target + r) < 0.f)) {
-      if (j.x) load4(j.x + r * j.ld + c, left, vec, v[i]);
-      else kept4(j.kept, r, c, v[i]);
-      if (j.act) {
+    for (int i = 0; i < 8; ++i) {
+      const float4 t = live[i] ? __ldg(reinterpret_cast<const float4 *>(j.x + (row0 + 16 * i) * j.ld + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[i][0] = t.x; v[i][1] = t.y; v[i][2] = t.z; v[i][3] = t.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[i][u] = live[i] && u < left ? __ldg(j.x + (row0 + 16 * i) * j.ld + c + u) : 0.f;
+  }
+  if (!PLAIN && j.act) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (live[i]) {
         float o[4];
-        if (j.out) load4(j.out + r * j.cols + c, left, vec_out, o);
-        else kept4(j.out_kept, r, c, o);
+        if (j.out) load4(j.out + (row0 + 16 * i) * j.cols + c, left, vec_out, o);
+        else kept4(j.out_kept, row0 + 16 * i, c, o);
 #pragma unroll
         for (int u = 0; u < 4; ++u) v[i][u] = u < left ? v[i][u] * act_bwd(j.act, o[u]) : 0.f;
       }
     }
+  }
+  uint32_t best = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
 #pragma unroll
     for (int u = 0; u < 4; ++u) best = max(best, finite_bits(v[i][u]));
-  }
-  if (j.keep.q) {
+  if (!PLAIN && j.keep.q) {
     // the 8-bit form (keep8.cu): 8 lanes share a scale
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int64_t r = (int64_t)rb * HALF_BLOCK + w + 16 * i;
+      const int64_t r = row0 + 16 * i;
       uint32_t mx = 0;
 #pragma unroll
       for (int u = 0; u < 4; ++u) mx = max(mx, finite_bits(v[i][u]));
@@ -633,7 +651,7 @@ __global__ void __launch_bounds__(512, 2) half_split_kernel(const __grid_constan
       }
     }
   }
-  if (j.hi) {
+  if (PLAIN || j.hi) {
     best = __reduce_max_sync(0xffffffffu, best);
     if (lane == 0) wmax[w] = best;
     __syncthreads();
@@ -643,17 +661,17 @@ __global__ void __launch_bounds__(512, 2) half_split_kernel(const __grid_constan
     const float s = pow2f_exact(ex);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int64_t r = (int64_t)rb * HALF_BLOCK + w + 16 * i;
+      const int64_t r = row0 + 16 * i;
       if (r < j.rows && left > 0) {        // (ld_out covers whole groups of 4)
         __half h[4], l[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) half_pair(v[i][u] * s, h[u], l[u]);
         *reinterpret_cast<uint2 *>(j.hi + r * j.ld_out + c) = *reinterpret_cast<uint2 *>(h);
-        if (j.lo) *reinterpret_cast<uint2 *>(j.lo + r * j.ld_out + c) = *reinterpret_cast<uint2 *>(l);
+        if (PLAIN || j.lo) *reinterpret_cast<uint2 *>(j.lo + r * j.ld_out + c) = *reinterpret_cast<uint2 *>(l);
       }
     }
   }
-  if (j.sums) {
+  if (!PLAIN && j.sums) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       float t = v[0][u];
@@ -676,6 +694,7 @@ static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 int launch_half_split(const HalfJob *jobs, int n, cudaStream_t s) {
   HalfJobs a;
+  bool plain = true;
   int64_t grid = 0;
   a.n = 0;
   for (int i = 0; i < n; ++i) {
@@ -685,11 +704,13 @@ int launch_half_split(const HalfJob *jobs, int n, cudaStream_t s) {
     a.vec_out[a.n] = aligned16(jobs[i].out) && jobs[i].cols % 4 == 0;
     a.begin[a.n] = (int)grid;
     grid += half_blocks(jobs[i].rows) * half_blocks(jobs[i].cols);
+    plain = plain && jobs[i].x && jobs[i].hi && jobs[i].lo && !jobs[i].act && !jobs[i].keep.q && !jobs[i].sums;
     ++a.n;
   }
   if (grid == 0) return ENDIA_B200_OK;
   EB_REQUIRE(grid < ((int64_t)1 << 31), ENDIA_B200_ELIMIT, "fp16-pair product: operands of more than 2^45 elements");
-  half_split_kernel<<<(unsigned)grid, 512, 0, s>>>(a);
+  if (plain) half_split_kernel<true><<<(unsigned)grid, 512, 0, s>>>(a);
+  else half_split_kernel<false><<<(unsigned)grid, 512, 0, s>>>(a);
   EB_LAUNCH_CHECK();
   return ENDIA_B200_OK;
 }

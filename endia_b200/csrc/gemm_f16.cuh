@@ -5,7 +5,8 @@
 // hi and lo hold 22 bits of every element down to 2^-15 of the largest one of its block; smaller ones are
 // exact to 2^-40 of it.  a*b = a_hi*b_hi + a_lo*b_hi + a_hi*b_lo (+ a_lo*b_lo, 2^-24 of the product, dropped).
 // The blocks' scales come out again where the accumulators are added in fp32: a run of 64 or 128 of K lies in one
-// block of each operand. A scale per array would need the array's maximum first, one more pass over it.
+// block of each operand, and a tile's sums are held in units of its largest product of unscaling factors (what
+// lies 2^-126 below that drops out). A scale per array would need the array's maximum first, one more pass.
 #pragma once
 #include "common.cuh"
 #include <cuda_fp16.h>
@@ -131,7 +132,7 @@ __device__ __forceinline__ void alpha_factors(const float *alpha, int extra, flo
       m = __uint_as_float((__float_as_uint(m) & 0x807FFFFFu) | 0x3F800000u);
     }
   }
-  const int e0 = e / 2, e1 = e - e0;
+  const int e0 = max(-126, min(126, e / 2)), e1 = max(-126, min(127, e - e0));
   f0 = m * pow2f_exact(e0);
   f1 = pow2f_exact(e1);
 }
