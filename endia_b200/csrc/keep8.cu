@@ -15,7 +15,6 @@
 // Replaces, for such a layer, the products of matmul_vjp and the masks of relu/tanh/sigmoid
 // (endia/functional/binary_ops/matmul_op.mojo:278-284, relu_op.mojo:95, tanh_op.mojo:92, sigmoid_op.mojo:98).
 #include "gemm_f16.cuh"
-#include "gemm.cuh"
 
 using namespace eb;
 

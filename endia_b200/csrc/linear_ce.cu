@@ -11,14 +11,14 @@
 // The reference's one loss is mse (endia/functional/loss_ops/mse_op.mojo:18-20); this is the
 // classification loss beside it.
 #include "gemm_f16.cuh"
-#include "gemm.cuh"
 #include <math.h>
 
 using namespace eb;
 
 namespace eb {
 
-// state: [0] rows that count, [1] CTAs of ce_rows_kernel that are done, [4 ...) lse per row, then lse log2 e per row. Inside, logits are in units of log2 e: exponentials are powers of two.
+// state: [0] rows that count, [1] CTAs of ce_rows_kernel that are done, [4 ...) lse per row, then lse log2 e per
+// row. Inside, logits are in units of log2 e: exponentials are powers of two.
 constexpr double CE_LOG2E = 1.4426950408889634, CE_LN2 = 0.6931471805599453;
 constexpr int CE_STATE_HEAD = 4;
 // Work space for one piece of the vocabulary (the d pair and W's pair, 4 bytes each per element).
