@@ -14,7 +14,7 @@
 // 1e-5 at K = 4096, at 3 fp16 MMAs per product (tf32 + 2 bf16 take the time of 4).
 //   warp 0: TMA producer (one lane), warp 1: MMA issuer (one lane of the leader CTA), warps 2, 3 idle
 //   warps 4-11: sums, epilogue and stores (lane quarter warp & 3, column half (warp - 4) >> 2)
-// The 168 registers a thread that the launch hands out are split as 56 for the first warpgroup and 224
+// The 168 registers a thread that the launch hands out are split as 40 for the first warpgroup and 232
 // for the other two (128 sums, 64 in flight from tensor memory).
 // Every wait is bounded; a wait that gives up records a code, the CTA drains its copies and returns.
 #include "gemm_f16.cuh"
@@ -27,7 +27,7 @@ constexpr int F16_BK = 64;                       // one stage: 64 of K, 128 byte
 constexpr uint32_t F16_TILE = 128 * F16_BK * 2;  // bytes of one [128 x 64] fp16 tile
 constexpr int F16_EPI_WARPS = 8;
 constexpr int F16_THREADS = 384;
-constexpr int F16_REGS_CONTROL = 56, F16_REGS_EPI = 224;
+constexpr int F16_REGS_CONTROL = 40, F16_REGS_EPI = 232;
 static_assert(F16_REGS_CONTROL * 128 + F16_REGS_EPI * 256 <= 168 * F16_THREADS, "registers of the launch");
 
 struct F16Maps {
@@ -108,6 +108,23 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+// Two fp32 lanes per instruction: (a0, a1) = (x0, x1) * s + (a0, a1), and products and sums of the kind.
+__device__ __forceinline__ void fma2(float &a0, float &a1, float x0, float x1, float s) {
+  asm("{\n\t.reg .b64 a, x, f;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 x, {%2, %3};\n\tmov.b64 f, {%4, %4};\n\t"
+      "fma.rn.f32x2 a, x, f, a;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(a0), "+f"(a1) : "f"(x0), "f"(x1), "f"(s));
+}
+__device__ __forceinline__ void scale_add2(float &a0, float &a1, float s, float b0, float b1) {      // a = a * s + b
+  asm("{\n\t.reg .b64 a, b, f;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%3, %4};\n\tmov.b64 f, {%2, %2};\n\t"
+      "fma.rn.f32x2 a, a, f, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(a0), "+f"(a1) : "f"(s), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void mul2(float &a0, float &a1, float s) {
+  asm("{\n\t.reg .b64 a, f;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 f, {%2, %2};\n\tmul.rn.f32x2 a, a, f;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}" : "+f"(a0), "+f"(a1) : "f"(s));
+}
+__device__ __forceinline__ void add2(float &a0, float &a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 a, a, b;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}" : "+f"(a0), "+f"(a1) : "f"(b0), "f"(b1));
 }
 __device__ __forceinline__ void sts128u(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -284,9 +301,9 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
             if (lane == 0) mbar_arrive_remote(empty_leader[b]);
           }
 #pragma unroll
-          for (int u = 0; u < 32; ++u) {
-            acc[32 * c + u] = fmaf(__uint_as_float(r0[u]), s0, acc[32 * c + u]);
-            acc[32 * c + 32 + u] = fmaf(__uint_as_float(r1[u]), s0, acc[32 * c + 32 + u]);
+          for (int u = 0; u < 32; u += 2) {
+            fma2(acc[32 * c + u], acc[32 * c + u + 1], __uint_as_float(r0[u]), __uint_as_float(r0[u + 1]), s0);
+            fma2(acc[32 * c + 32 + u], acc[32 * c + 33 + u], __uint_as_float(r1[u]), __uint_as_float(r1[u + 1]), s0);
           }
         }
         ++j;
@@ -407,7 +424,13 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
               for (int i = 0; i < 32; ++i) v[i] = exp2_fast(fmaf(acc[32 * c + i], to_log2, __shfl_sync(0xffffffffu, bv[c], i) - lse));
             } else {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = exp2_fast(fmaf(acc[32 * c + i], to_log2, -lse));
+              for (int i = 0; i < 32; i += 2) {
+                v[i] = acc[32 * c + i];
+                v[i + 1] = acc[32 * c + i + 1];
+                scale_add2(v[i], v[i + 1], to_log2, -lse, -lse);
+                v[i] = exp2_fast(v[i]);
+                v[i + 1] = exp2_fast(v[i + 1]);
+              }
             }
             if (any_target) {
 #pragma unroll
@@ -415,7 +438,7 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
                 if (32 * c + i == tl) v[i] -= 1.f;
             }
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] *= cs;
+            for (int i = 0; i < 32; i += 2) mul2(v[i], v[i + 1], cs);
             if (any_dead) {      // rows that are left out: exactly zero, whatever their logits are
 #pragma unroll
               for (int i = 0; i < 32; ++i) v[i] = cf == 0.f ? 0.f : v[i];
@@ -425,7 +448,9 @@ gemm_f16_kernel(const __grid_constant__ F16Maps maps, const F16Params p) {
             for (int u = 0; u < 16; ++u) {
               const __half2 h = __floats2half2_rn(v[2 * u], v[2 * u + 1]);
               const float2 hf = __half22float2(h);
-              const __half2 l = __floats2half2_rn(v[2 * u] - hf.x, v[2 * u + 1] - hf.y);
+              float l0 = v[2 * u], l1 = v[2 * u + 1];
+              add2(l0, l1, -hf.x, -hf.y);
+              const __half2 l = __floats2half2_rn(l0, l1);
               hi[u] = *reinterpret_cast<const uint32_t *>(&h);
               lo[u] = *reinterpret_cast<const uint32_t *>(&l);
             }
