@@ -6,7 +6,8 @@
 // exponentials (8 bytes instead of 512); a second kernel joins them per row. Backward: per piece of the
 // vocabulary the logits are formed again, d leaves the epilogue as an fp16 pair (|d| <= 1, a fixed
 // scale), and feeds the two gradient products of the piece. 8 M K V multiply-adds instead of the 6
-// that kept logits would take, at 4 (M + K) bytes of work space per column of a piece.
+// that kept logits would take, at 4 (M + K) bytes of work space per column of a piece. A step of 2048 x 1024 x
+// 32768 takes 1.54 ms (265 us statistics, per piece 166 us d, 148 us dx, 157 us dW, 25 us for the pairs of W).
 // The products run on the fp16-pair tensor-core kernel (gemm_f16.cuh), but the forward one of up to 16 rows.
 // The reference's one loss is mse (endia/functional/loss_ops/mse_op.mojo:18-20); this is the
 // classification loss beside it.
@@ -21,7 +22,8 @@ namespace eb {
 // row. Inside, logits are in units of log2 e: exponentials are powers of two.
 constexpr double CE_LOG2E = 1.4426950408889634, CE_LN2 = 0.6931471805599453;
 constexpr int CE_STATE_HEAD = 4;
-// Work space for one piece of the vocabulary (the d pair and W's pair, 4 bytes each per element).
+// Work space for one piece of the vocabulary (the d pair and W's pair, 4 bytes each per element). Smaller
+// pieces cost rounds of tiles: 128 MiB 7 %, 64 MiB 22 % more time at 2048 x 1024 x 32768.
 constexpr int64_t CE_PIECE_BYTES = (int64_t)256 << 20;
 constexpr int64_t CE_MIN_PIECE = 1024;
 constexpr int CE_MAX_CLASSES = 1 << 24;    // class numbers are float32 values
@@ -129,7 +131,8 @@ ce_coef_kernel(const float *__restrict__ g, int per_row, int mean, const float *
 // The statistics of up to 16 rows in one pass over W, which is all that such a call has to read: a CTA takes 128
 // columns, its eight warps take the features in turn (x as [feature][row] in shared memory, four columns
 // and ROWS x 4 sums a lane), and eight to sixteen loads of 128 bits a lane are in flight. The warps' sums are added in
-// order, then a warp per row (two rows) reduces 128 logits as the tensor-core epilogue does.
+// order, then a warp per row (two rows) reduces 128 logits as the tensor-core epilogue does. 8 rows at
+// 1024 x 32768: 39 us cold (134 MB, 3.4 TB/s), against 133 us for the product of few rows of gemm_skinny.cu and its reduction.
 constexpr int CE_FEW = 16, CE_FEW_K = 512;
 template <int ROWS, bool VEC>
 __global__ void __launch_bounds__(256)
