@@ -111,9 +111,9 @@ struct Carver {       // a caller's work space, handed out in 256-byte steps (ba
 };
 
 // Scale exponent of a block from its largest finite |x|: 14 - floor(log2 amax), at most 126 (a block of
-// values below 2^-112 keeps fewer than 22 bits, down to those of a denormal).
+// values below 2^-112 keeps fewer than 22 bits, down to those of a denormal). A block of zeros has 126: it must
+// not set the unit of a tile whose other blocks are tiny.
 __host__ __device__ __forceinline__ int half_scale_exponent(uint32_t amax_bits) {
-  if (amax_bits == 0) return 0;
   const int ex = 141 - (int)(amax_bits >> 23);
   return ex > 126 ? 126 : ex;
 }

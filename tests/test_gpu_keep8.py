@@ -315,6 +315,29 @@ def test_second_order_through_a_checkpointed_layer(nd):
     assert np.abs(dw - want).max() <= 1e-4 * np.abs(want).max()
 
 
+@pytest.mark.parametrize("sx,sw", [(1e-19, 1e-18), (1e-37, 1.0), (1e18, 1e-18), (1e25, 1e-30)])
+def test_blocks_of_zeros_beside_tiny_and_large_ones(nd, sx, sw):
+    """The operands have a scale per block of 128 x 128; one that is all zeros says nothing about the others,
+    and products across blocks of far-apart scales keep the bounds."""
+    x, w, b, g = layer_case(300, 390, 260, 31)
+    x, w = (x * sx).astype(np.float32), (w * sw).astype(np.float32)
+    x[:, :128] = 0
+    w[128:256] = 0
+    x[130:256, 256:] *= np.float32(2.0 ** -20)
+    X, W = nd.Array(x, requires_grad=True), nd.Array(w, requires_grad=True)
+    out = nd.nn.linear(X, W, checkpoint=True)
+    x64, w64 = x.astype(np.float64), w.astype(np.float64)
+    size = np.abs(x64) @ np.abs(w64)
+    floor = 2.0 ** -38 * np.abs(x).max() * np.abs(w).max() * 390 + 1e-44
+    assert (np.abs(out.to_numpy() - x64 @ w64) <= (12 + 390 / 64) * U * size + floor).all()
+    assert np.abs(out.to_numpy()).max() > 0
+    nd.sum(out * nd.Array(g)).backward()
+    xk = kept_values(x, False)
+    for got, ref, mag, n in ((X.grad(), g @ w64.T, np.abs(g) @ np.abs(w64).T, 260), (W.grad(), xk.T @ g, np.abs(xk).T @ np.abs(g), 300)):
+        tiny = 2.0 ** -38 * np.abs(g).max() * (np.abs(w).max() if n == 260 else np.abs(xk).max()) * n + 1e-44
+        assert (np.abs(got.to_numpy() - ref) <= (27 + n / 64) * U * mag + tiny).all()
+
+
 def test_jacobian_of_a_checkpointed_layer(nd):
     x, w, b, _ = layer_case(3, 5, 4, 21)
     X, W, B = (nd.Array(a, requires_grad=True) for a in (x, w, b))
