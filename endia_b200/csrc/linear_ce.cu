@@ -8,7 +8,8 @@
 // scale), and feeds the two gradient products of the piece. 8 M K V multiply-adds instead of the 6
 // that kept logits would take, at 4 (M + K) bytes of work space per column of a piece. A step of 2048 x 1024 x
 // 32768 takes 1.54 ms (265 us statistics, per piece 166 us d, 148 us dx, 157 us dW, 25 us for the pairs of W).
-// The products run on the fp16-pair tensor-core kernel (gemm_f16.cuh), but the forward one of up to 16 rows.
+// The products run on the fp16-pair tensor-core kernel (gemm_f16.cuh), but that of up to 16 rows
+// without a backward pass.
 // The reference's one loss is mse (endia/functional/loss_ops/mse_op.mojo:18-20); this is the
 // classification loss beside it.
 #include "gemm_f16.cuh"
@@ -240,9 +241,11 @@ static int launch_few_rows(const float *x, int64_t ldx, const float *W, int64_t 
   return ENDIA_B200_OK;
 }
 
-// Up to 16 rows the forward pass reads W once and is done (4 bytes per weight; making pairs first costs 16);
-// its multiply-adds stay below the time of that read on the fp32 pipes.
-static bool ce_few_rows(int64_t M) { return M <= CE_FEW; }
+// Up to 16 rows a forward pass that no backward pass follows reads W once and is done (4 bytes per weight; making
+// pairs first costs 16); its multiply-adds stay below the time of that read on the fp32 pipes. Where a
+// backward pass follows, both take the logits from the same kernel: their common error (4e-7 of a logit,
+// always towards zero) then cancels in l - lse; against an fp32 lse it stays (1.3e-6 of dx at 8 x 3584 x 640).
+static bool ce_few_rows(int64_t M, bool alone) { return alone && M <= CE_FEW; }
 
 // Columns per piece: equal pieces (multiples of 256) whose work space stays near CE_PIECE_BYTES.
 static int64_t ce_piece(int64_t bytes_per_column, int64_t V) {
@@ -252,13 +255,14 @@ static int64_t ce_piece(int64_t bytes_per_column, int64_t V) {
   return ceil_div(ceil_div(V, pieces), 256) * 256;
 }
 
-struct CeForward { float2 *stats; float *tl, *rows; __half *xh, *xl, *wh, *wl; int *xe, *we; int64_t piece, parts, ldx; };
-static size_t ce_carve_forward(int64_t M, int64_t K, int64_t V, char *base, CeForward &f) {
+struct CeForward { float2 *stats; float *tl, *rows, *state; __half *xh, *xl, *wh, *wl; int *xe, *we; int64_t piece, parts, ldx; };
+static size_t ce_carve_forward(int64_t M, int64_t K, int64_t V, bool alone, char *base, CeForward &f) {
   Carver c{base};
   f = CeForward{};
   f.tl = c.take<float>(M);
   f.rows = c.take<float>(M);
-  if (ce_few_rows(M)) {
+  if (alone) f.state = c.take<float>(CE_STATE_HEAD + 2 * M);
+  if (ce_few_rows(M, alone)) {
     f.parts = ceil_div(V, 128);
   } else {
     f.piece = ce_piece(4 * K, V);
@@ -324,11 +328,11 @@ extern "C" {
 
 size_t endia_b200_linear_ce_state_bytes(int64_t M) { return M < 0 ? 0 : sizeof(float) * (size_t)(CE_STATE_HEAD + 2 * M); }
 
-size_t endia_b200_linear_ce_scratch_bytes(int64_t M, int64_t K, int64_t V, int32_t backward) {
+size_t endia_b200_linear_ce_scratch_bytes(int64_t M, int64_t K, int64_t V, int32_t pass) {
   if (M <= 0 || K <= 0 || V <= 0 || V > CE_MAX_CLASSES || M > (1 << 27) || K > (1 << 27)) return 256;
   CeForward f;
   CeBackward b;
-  return backward ? ce_carve_backward(M, K, V, nullptr, b) : ce_carve_forward(M, K, V, nullptr, f);
+  return pass == 1 ? ce_carve_backward(M, K, V, nullptr, b) : ce_carve_forward(M, K, V, pass == 2, nullptr, f);
 }
 
 int endia_b200_linear_ce_fwd(const float *x, int64_t ldx, const float *W, int64_t ldw, const float *bias,
@@ -337,18 +341,21 @@ int endia_b200_linear_ce_fwd(const float *x, int64_t ldx, const float *W, int64_
   int st = require_device();
   if (st) return st;
   if ((st = ce_check(x, ldx, W, ldw, target, M, K, V, reduction, scratch))) return st;
-  EB_REQUIRE(state && scratch && (loss || (reduction == ENDIA_B200_LOSS_NONE && M == 0)), ENDIA_B200_EINVAL,
-             "linear_ce: loss, state and scratch are required");
+  EB_REQUIRE(scratch && (loss || (reduction == ENDIA_B200_LOSS_NONE && M == 0)), ENDIA_B200_EINVAL,
+             "linear_ce: loss and scratch are required");
   cudaStream_t s = as_stream(stream);
-  EB_CUDA(cudaMemsetAsync(state, 0, CE_STATE_HEAD * sizeof(float), s));
+  const bool alone = state == nullptr;
+  CeForward f;
+  ce_carve_forward(M, K, V, alone, static_cast<char *>(scratch), f);
+  if (alone) state = f.state;
   if (M == 0) {
+    if (!alone) EB_CUDA(cudaMemsetAsync(state, 0, CE_STATE_HEAD * sizeof(float), s));
     if (reduction != ENDIA_B200_LOSS_NONE) EB_CUDA(cudaMemsetAsync(loss, 0, sizeof(float), s));
     return ENDIA_B200_OK;
   }
-  CeForward f;
-  ce_carve_forward(M, K, V, static_cast<char *>(scratch), f);
+  EB_CUDA(cudaMemsetAsync(state, 0, CE_STATE_HEAD * sizeof(float), s));
   float *rows = reduction == ENDIA_B200_LOSS_NONE ? loss : f.rows;
-  if (ce_few_rows(M)) {
+  if (ce_few_rows(M, alone)) {
     const auto few = M <= 1 ? launch_few_rows<1> : M <= 2 ? launch_few_rows<2> : M <= 4 ? launch_few_rows<4>
                      : M <= 8 ? launch_few_rows<8> : launch_few_rows<CE_FEW>;
     if ((st = few(x, ldx, W, ldw, bias, target, (int)M, (int)K, (int)V, f.stats, f.tl, s))) return st;

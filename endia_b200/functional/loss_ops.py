@@ -141,11 +141,12 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean"):
     def call(curr, a):
         setup_shape_and_data(curr)
         hold, ops = operands(a)
-        state = alloc(_lib.lib.endia_b200_linear_ce_state_bytes(M) // 4)
-        scratch = _scratch(_lib.lib.endia_b200_linear_ce_scratch_bytes(M, K, V, 0))
-        _lib.call("endia_b200_linear_ce_fwd", *ops, curr.data_ptr(), state.data_ptr(), scratch.data_ptr(), stream())
+        state = None
         if curr.requires_grad_flag:
-            saved["state"] = state
+            state = saved["state"] = alloc(_lib.lib.endia_b200_linear_ce_state_bytes(M) // 4)
+        scratch = _scratch(_lib.lib.endia_b200_linear_ce_scratch_bytes(M, K, V, 0 if state is not None else 2))
+        _lib.call("endia_b200_linear_ce_fwd", *ops, curr.data_ptr(), state.data_ptr() if state is not None else None,
+                  scratch.data_ptr(), stream())
 
     def state_array(shape, offset):
         arr = Array(ArrayShape(shape, None, offset))

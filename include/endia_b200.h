@@ -325,17 +325,17 @@ enum { ENDIA_B200_LOSS_MEAN = 0, ENDIA_B200_LOSS_SUM = 1, ENDIA_B200_LOSS_NONE =
  *   reduction MEAN: loss[0] = sum / number of rows that count (0 when none does);  SUM: loss[0] = sum;
  *   NONE: loss[M], one per row
  * `state` (endia_b200_linear_ce_state_bytes(M) bytes) carries what the backward call needs besides the
- * inputs (log-sum-exp per row, the count, the operands' scales); x, W, bias and target must be
- * unchanged then. `grad` is the incoming gradient: one float (MEAN, SUM) or M floats (NONE).
+ * inputs (log-sum-exp per row, the count); x, W, bias and target must be unchanged then. NULL: no backward
+ * call follows (up to 16 rows then take one fp32 pass over W). `grad` is the incoming gradient: one float (MEAN, SUM) or M floats (NONE).
  *   dx [M, K], dw [K, V], db [V], all contiguous, each may be NULL (not computed)
- * `scratch`: endia_b200_linear_ce_scratch_bytes(M, K, V, backward) bytes, 256-byte aligned: the
- * vocabulary is walked in equal pieces whose work space stays near 256 MiB (pieces of at least 1024
+ * `scratch`: endia_b200_linear_ce_scratch_bytes(M, K, V, pass) bytes, 256-byte aligned (pass 0: forward, 1:
+ * backward, 2: forward with state == NULL): the vocabulary is walked in equal pieces whose work space stays near 256 MiB (pieces of at least 1024
  * columns), beside 4 bytes per element of x and, forward, 8 bytes per row and 128 classes. Limits: V <= 2^24 (class numbers are float32 values), M and K below 2^27. The order of
  * every sum is fixed: the same inputs give the same bits.
- * Accuracy: products of 22-bit operand pairs summed in fp32 (fp32 kernels for small problems).
+ * Accuracy: products of 22-bit operand pairs summed in fp32.
  * No counterpart in the reference, whose one loss is mse (endia/functional/loss_ops/mse_op.mojo:18-20). */
 size_t endia_b200_linear_ce_state_bytes(int64_t M);
-size_t endia_b200_linear_ce_scratch_bytes(int64_t M, int64_t K, int64_t V, int32_t backward);
+size_t endia_b200_linear_ce_scratch_bytes(int64_t M, int64_t K, int64_t V, int32_t pass);
 int endia_b200_linear_ce_fwd(const float *x, int64_t ldx, const float *W, int64_t ldw, const float *bias,
                              const float *target, int64_t M, int64_t K, int64_t V, int32_t reduction, float *loss,
                              float *state, void *scratch, void *stream);

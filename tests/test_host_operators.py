@@ -91,6 +91,9 @@ def test_work_space_sizes():
         small, large = (lib.endia_b200_linear_ce_scratch_bytes(M, K, v, back) for v in (1 << 15, 1 << 19))
         assert large - small <= 4 * M * ((1 << 19) - (1 << 15)) // 64 + (160 << 20), back
         assert large < (900 << 20) < 4 * M * (1 << 19)
+    # up to 16 rows without a backward pass: no pairs
+    assert lib.endia_b200_linear_ce_scratch_bytes(16, 4096, 1 << 17, 2) < (1 << 20)
+    assert lib.endia_b200_linear_ce_scratch_bytes(17, 4096, 1 << 17, 2) > (1 << 20)
     # piece floor: many rows
     assert lib.endia_b200_linear_ce_scratch_bytes(1 << 20, 64, 1 << 17, 1) < 4 * (1 << 20) * (1 << 17) // 16
 
